@@ -424,6 +424,68 @@ MA_API int ma_prefix_attention_gather(const ma_rows* q, const ma_kv* kv, int H, 
                                       int world, int rank, void* const* regions, int Tg, void* gout,
                                       const int64_t sgo[3], void* gather_ws, size_t gather_ws_bytes, void* stream);
 
+/* ---- paged serving --------------------------------------------------------------------
+ * What a serving loop over a paged token-mode k4v4 cache does per step beside the select +
+ * attend path (the reference has neither pages nor a batch loop): plan the step's slots,
+ * append the new tokens, attend with few rows, verify drafted tokens.
+ *
+ * ma_page_plan: page tables and slot maps from the requests' lengths lens [B] (now) and
+ *   new_lens [B] (wanted), int32. pages [B, width] (row stride spg) holds each request's
+ *   pool pages, ceil(lens / page_size) of them; free_list [num_pages] is a stack of
+ *   free_count[0] unused pages. A shorter request hands its last pages back (onto the stack,
+ *   in (request, page) order), a longer one takes pages from the top. Requests grow in
+ *   their order while the free pages (those handed back included) and max_tokens last; from
+ *   the first that does not fit on, none grows and its length stays (so lens_out != new_lens
+ *   there); one that would not fit its table keeps its length alone. Negative lengths count
+ *   as 0. Written: lens_out [B], pages_out [B, width] (entries past a request's pages keep
+ *   what `pages` has), free_out, free_count_out, starts [B + 1] (first new token of each
+ *   request) and for the N = starts[B] new tokens slots (page * page_size + offset; -1 on
+ *   a page number outside [0, num_pages)), seqs (the request) and positions, each
+ *   [max_tokens] with -1 from N on. Every output may be its input (in place); those three
+ *   arrays are 16-byte aligned. B above 8192 returns MA_ERR_UNSUPPORTED.
+ * ma_append_tokens: N tokens' rows k, v [N, H, D] (strides over (token, head)) quantized as
+ *   ma_quantize_tokens does (keys divided by kchan of sequence seqs[i]) into slots[i] of the
+ *   pool (a paged token-mode ma_kv without tail; its page table is not read). A token whose
+ *   slot lies outside the pool or whose sequence lies outside [0, B) is not stored; two
+ *   tokens of one call must not name the same slot. k_rows / v_rows [N, H, D] contiguous
+ *   (optional, in `dtype`): the values the slots stand for, code * scale + zero (* kchan)
+ *   rounded once; zeros for a sequence outside [0, B).
+ * ma_decode_attention: ma_prefix_attention's output for few rows over a token-mode k4v4 cache
+ *   without tail (contiguous or paged, lens, mask) read in place, its elements not rounded
+ *   to bf16 on the way, and over the step's own keys: with `causal`, row t sees block key
+ *   j iff j <= t + Tc - T (Tc >= T), else every block key. A row without any key is zero.
+ *   bf16 rows; scale and zero rows aligned to their D/16 bytes; other layouts return
+ *   MA_ERR_UNSUPPORTED (ma_prefix_attention serves them). Any R = G*T, 32 rows per pass over
+ *   the cache.
+ * ma_verify_drafts: K drafted tokens per request (tokens [B, K] contiguous, counts [B] of them
+ *   in use, NULL = K) against the target's probabilities target [B, K + 1, V] and the
+ *   drafter's draft [B, K, V] (strides over (request, position), vocabulary contiguous;
+ *   MA_F32, MA_BF16 or MA_F16; draft NULL: each draft was certain) with uniforms [B, K + 1]
+ *   in [0, 1). Draft i is accepted while u_i q_i(x_i) < p_i(x_i) (one fp32 product; a token
+ *   outside [0, V) is refused); accepted [B] = the run a. The next token is drawn from
+ *   max(p_a - q_a, 0), or p_a when all counts[b] drafts were accepted or no residual mass is
+ *   left: with w_v = floor(min(r_v, 1) 2^40) and U = floor(u_K 2^24) it is the first v whose
+ *   inclusive sum exceeds floor(U sum(w) / 2^24) -- whole numbers, so the same token whatever
+ *   the order of the sums; -1 if p_a has no mass. out [B, K + 1]: the accepted drafts, the
+ *   next token, then -1. V above 2^20 or B above 65535 returns MA_ERR_UNSUPPORTED.       */
+MA_API size_t ma_page_plan_workspace(void);
+MA_API int ma_page_plan(const int32_t* lens, const int32_t* new_lens, int B, const int32_t* pages, int64_t spg,
+                        int width, const int32_t* free_list, const int32_t* free_count, int num_pages, int page_size,
+                        int max_tokens, int32_t* lens_out, int32_t* pages_out, int64_t spg_out, int32_t* free_out,
+                        int32_t* free_count_out, int32_t* starts, int64_t* slots, int32_t* seqs, int32_t* positions,
+                        void* workspace, size_t workspace_bytes, void* stream);
+MA_API int ma_append_tokens(const ma_kv* pool, int B, int H, int D, const void* k, const void* v, int32_t dtype, int N,
+                            const int64_t sk[2], const int64_t sv[2], const int64_t* slots, const int32_t* seqs,
+                            void* k_rows, void* v_rows, void* stream);
+MA_API size_t ma_decode_attention_workspace(int B, int H, int R, int D, int Tc);
+MA_API int ma_decode_attention(const ma_rows* q, const ma_kv* kv, int H, const ma_block* cur, float scale, int causal,
+                               void* out, const int64_t so[3], void* workspace, size_t workspace_bytes, void* stream);
+MA_API size_t ma_verify_drafts_workspace(int B, int V);
+MA_API int ma_verify_drafts(const void* target, const void* draft, int32_t dtype, int B, int K, int V,
+                            const int64_t st[2], const int64_t sd[2], const int32_t* tokens, const int32_t* counts,
+                            const float* uniforms, int32_t* accepted, int32_t* out, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -124,6 +124,17 @@ _SIGNATURES = {
     "ma_prefix_attention_gather": (_i32, [_P(MaRows), _P(MaKV), _i32, _P(MaBlock), _f32, _i32, _i32, _i32,
                                           _vp, _P(ctypes.c_int64), _vp, _vp, _vp, _vp, _sz, _i32, _i32, _P(_vp),
                                           _i32, _vp, _P(ctypes.c_int64), _vp, _sz, _vp]),
+    "ma_page_plan_workspace": (_sz, []),
+    "ma_page_plan": (_i32, [_vp, _vp, _i32, _vp, ctypes.c_int64, _i32, _vp, _vp, _i32, _i32, _i32, _vp, _vp,
+                            ctypes.c_int64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "ma_append_tokens": (_i32, [_P(MaKV), _i32, _i32, _i32, _vp, _vp, _i32, _i32, _P(ctypes.c_int64),
+                                _P(ctypes.c_int64), _vp, _vp, _vp, _vp, _vp]),
+    "ma_decode_attention_workspace": (_sz, [_i32] * 5),
+    "ma_decode_attention": (_i32, [_P(MaRows), _P(MaKV), _i32, _P(MaBlock), _f32, _i32, _vp, _P(ctypes.c_int64),
+                                   _vp, _sz, _vp]),
+    "ma_verify_drafts_workspace": (_sz, [_i32, _i32]),
+    "ma_verify_drafts": (_i32, [_vp, _vp, _i32, _i32, _i32, _i32, _P(ctypes.c_int64), _P(ctypes.c_int64), _vp, _vp,
+                                _vp, _vp, _vp, _vp, _sz, _vp]),
 }
 
 EXPORTED = tuple(_SIGNATURES)

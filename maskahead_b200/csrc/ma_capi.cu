@@ -757,4 +757,211 @@ int ma_head_gather(const void* part, const int64_t sp[3], int B, int Hl, int T, 
                                 (cudaStream_t)stream);
 }
 
+// ------------------------------------------------------------------ paged serving
+namespace {
+
+// workspace: [256-byte aligned] error word block, then the CTA tickets (fixed-size blocks, so
+// their words do not move with a call's sizes), then the call's scratch
+constexpr size_t kDecodeTickets = 65536;
+constexpr size_t kVerifyTickets = 65536;
+
+inline char* align256(void* ws) {
+  return reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(ws) + 255) & ~uintptr_t(255));
+}
+
+size_t decode_scratch(int H, int D, const DecodePlan& d, size_t& ml) {
+  const size_t splits = (size_t)H * d.row_tiles * d.slots * d.rows;
+  ml = (splits * sizeof(float2) + 255) & ~(size_t)255;
+  return ml + splits * D * sizeof(float);
+}
+
+// a pool (or contiguous cache) of token-mode k4v4 rows without a dense tail whose scale and
+// zero rows a copy of their own size can read
+bool packed_in_place(const ma_kv& kv, int D) {
+  if (kv.layout != MA_KV_PACKED_TOKEN || kv.nf != 0) return false;
+  if (kv.nq == 0) return true;
+  const uintptr_t row = (uintptr_t)(D / 16), halves = row / 2;
+  uintptr_t bits = reinterpret_cast<uintptr_t>(kv.ks) | reinterpret_cast<uintptr_t>(kv.kz) |
+                   reinterpret_cast<uintptr_t>(kv.vs) | reinterpret_cast<uintptr_t>(kv.vz);
+  if (bits & (row - 1)) return false;
+  for (int i = 0; i < 3; ++i)
+    if (((uintptr_t)kv.sks[i] | (uintptr_t)kv.svs[i]) & (halves - 1)) return false;
+  return true;
+}
+
+}  // namespace
+
+size_t ma_decode_attention_workspace(int B, int H, int R, int D, int Tc) {
+  if (B <= 0 || H <= 0 || R <= 0 || D <= 0 || Tc < 0) return 0;
+  DecodePlan d;
+  plan_decode(B, H, R, Tc, d);
+  size_t ml;
+  return 512 + kDecodeTickets * sizeof(unsigned) + decode_scratch(H, D, d, ml);
+}
+
+int ma_decode_attention(const ma_rows* q, const ma_kv* kv, int H, const ma_block* cur, float scale, int causal,
+                        void* out, const int64_t so[3], void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_rows(q);
+  if (rc) return rc;
+  if (H <= 0 || q->Hq % H) return MA_ERR_ARG;
+  if ((rc = check_kv(kv, q->D))) return rc;
+  if ((rc = check_block(cur, q, H))) return rc;
+  if (!out || !so || !aligned16(out) || !strides16(so, 3, esize(q->dtype))) return MA_ERR_ARG;
+  if (causal && cur->Tc > 0 && cur->Tc < q->T) return MA_ERR_ARG;
+  if (q->dtype != MA_BF16 || kv->dtype != MA_BF16 || !packed_in_place(*kv, q->D)) return MA_ERR_UNSUPPORTED;
+  DecodeParams p;
+  p.G = q->Hq / H;
+  if ((int64_t)p.G * q->T > 0x7fffffffLL / 64) return MA_ERR_UNSUPPORTED;
+  p.R = p.G * q->T;
+  DecodePlan d;
+  plan_decode(q->B, H, p.R, cur->Tc, d);
+  if ((int64_t)H * d.row_tiles > 65535 || (int64_t)q->B * H * d.row_tiles > (int64_t)kDecodeTickets)
+    return MA_ERR_UNSUPPORTED;
+  size_t ml;
+  const size_t scratch = decode_scratch(H, q->D, d, ml);
+  if (!workspace || workspace_bytes < 512 + kDecodeTickets * sizeof(unsigned) + scratch) return MA_ERR_WORKSPACE;
+  char* base = align256(workspace) + 256;
+  p.q = reinterpret_cast<const __nv_bfloat16*>(q->q);
+  p.kv = *kv;
+  p.cur = *cur;
+  p.B = q->B;
+  p.H = H;
+  p.T = q->T;
+  p.D = q->D;
+  p.scale = scale;
+  p.causal = causal;
+  p.out = reinterpret_cast<__nv_bfloat16*>(out);
+  for (int i = 0; i < 3; ++i) {
+    p.sq[i] = q->sq[i];
+    p.so[i] = so[i];
+  }
+  p.tickets = reinterpret_cast<unsigned*>(base);
+  base += kDecodeTickets * sizeof(unsigned);
+  p.ml = reinterpret_cast<float2*>(base);
+  p.acc = reinterpret_cast<float*>(base + ml);
+  p.slots = d.slots;
+  p.target = d.target;
+  p.min_units = 1;
+  p.row_tiles = d.row_tiles;
+  return launch_decode_attention(p, (cudaStream_t)stream);
+}
+
+size_t ma_page_plan_workspace(void) { return 512; }
+
+int ma_page_plan(const int32_t* lens, const int32_t* new_lens, int B, const int32_t* pages, int64_t spg, int width,
+                 const int32_t* free_list, const int32_t* free_count, int num_pages, int page_size, int max_tokens,
+                 int32_t* lens_out, int32_t* pages_out, int64_t spg_out, int32_t* free_out, int32_t* free_count_out,
+                 int32_t* starts, int64_t* slots, int32_t* seqs, int32_t* positions, void* workspace,
+                 size_t workspace_bytes, void* stream) {
+  if (B <= 0 || width <= 0 || num_pages <= 0 || page_size <= 0 || max_tokens < 0) return MA_ERR_ARG;
+  if (!lens || !new_lens || !pages || !free_list || !free_count || !lens_out || !pages_out || !free_out ||
+      !free_count_out || !starts)
+    return MA_ERR_ARG;
+  if (max_tokens > 0 && (!slots || !seqs || !positions || !aligned16(slots) || !aligned16(seqs) || !aligned16(positions)))
+    return MA_ERR_ARG;
+  if (spg < width || spg_out < width || (pages == pages_out && spg != spg_out)) return MA_ERR_ARG;
+  if (B > page_plan_max_requests() || (int64_t)B * width > 0x7fffffffLL) return MA_ERR_UNSUPPORTED;
+  if (!workspace || workspace_bytes < ma_page_plan_workspace()) return MA_ERR_WORKSPACE;
+  PagePlanParams p;
+  p.lens = lens;
+  p.new_lens = new_lens;
+  p.pages = pages;
+  p.free_list = free_list;
+  p.free_count = free_count;
+  p.B = B;
+  p.width = width;
+  p.num_pages = num_pages;
+  p.page_size = page_size;
+  p.max_tokens = max_tokens;
+  p.spg = spg;
+  p.spg_out = spg_out;
+  p.lens_out = lens_out;
+  p.pages_out = pages_out;
+  p.free_out = free_out;
+  p.count_out = free_count_out;
+  p.starts = starts;
+  p.slots = slots;
+  p.seqs = seqs;
+  p.positions = positions;
+  p.ticket = reinterpret_cast<unsigned*>(align256(workspace) + 128);
+  p.pages_in_place = pages == pages_out ? 1 : 0;
+  p.free_in_place = free_list == free_out ? 1 : 0;
+  return launch_page_plan(p, (cudaStream_t)stream);
+}
+
+int ma_append_tokens(const ma_kv* pool, int B, int H, int D, const void* k, const void* v, int32_t dtype, int N,
+                     const int64_t sk[2], const int64_t sv[2], const int64_t* slots, const int32_t* seqs,
+                     void* k_rows, void* v_rows, void* stream) {
+  if (!pool || B <= 0 || H <= 0 || N < 0) return MA_ERR_ARG;
+  if (D != 64 && D != 128) return MA_ERR_UNSUPPORTED;
+  if (!valid_dtype(dtype)) return MA_ERR_ARG;
+  if (pool->layout != MA_KV_PACKED_TOKEN || pool->nf != 0) return MA_ERR_UNSUPPORTED;
+  if (pool->page_size <= 0 || pool->num_pages <= 0 || pool->nq <= 0) return MA_ERR_ARG;
+  int rc = check_kv(pool, D);
+  if (rc) return rc;
+  if (N == 0) return MA_OK;
+  if (!k || !v || !sk || !sv || !slots || !seqs || !aligned16(k) || !aligned16(v)) return MA_ERR_ARG;
+  if (!strides16(sk, 2, esize(dtype)) || !strides16(sv, 2, esize(dtype))) return MA_ERR_ARG;
+  if ((k_rows && !aligned16(k_rows)) || (v_rows && !aligned16(v_rows))) return MA_ERR_ARG;
+  if (pool->skc[0] < 0 || pool->skc[1] < 0) return MA_ERR_ARG;
+  AppendParams p;
+  p.k = k;
+  p.v = v;
+  for (int i = 0; i < 2; ++i) {
+    p.sk[i] = sk[i];
+    p.sv[i] = sv[i];
+  }
+  p.N = N;
+  p.B = B;
+  p.H = H;
+  p.D = D;
+  p.slots = slots;
+  p.seqs = seqs;
+  p.kv = *pool;
+  p.k_rows = k_rows;
+  p.v_rows = v_rows;
+  return launch_append_tokens(p, dtype, (cudaStream_t)stream);
+}
+
+size_t ma_verify_drafts_workspace(int B, int V) {
+  if (B <= 0 || V <= 0) return 0;
+  int chunk, chunks;
+  plan_verify(B, V, chunk, chunks);
+  return 512 + kVerifyTickets * sizeof(unsigned) + (size_t)B * chunks * sizeof(unsigned long long);
+}
+
+int ma_verify_drafts(const void* target, const void* draft, int32_t dtype, int B, int K, int V, const int64_t st[2],
+                     const int64_t sd[2], const int32_t* tokens, const int32_t* counts, const float* uniforms,
+                     int32_t* accepted, int32_t* out, void* workspace, size_t workspace_bytes, void* stream) {
+  if (B <= 0 || K < 0 || V <= 0 || !target || !st || !uniforms || !accepted || !out) return MA_ERR_ARG;
+  if (dtype != MA_F32 && dtype != MA_BF16 && dtype != MA_F16) return MA_ERR_ARG;
+  if (K > 0 && !tokens) return MA_ERR_ARG;
+  if (draft && K > 0 && (!sd || sd[0] < 0 || sd[1] < 0)) return MA_ERR_ARG;
+  if (st[0] < 0 || st[1] < 0) return MA_ERR_ARG;
+  const uintptr_t low = dtype == MA_F32 ? 3 : 1;
+  if ((reinterpret_cast<uintptr_t>(target) | reinterpret_cast<uintptr_t>(draft)) & low) return MA_ERR_ARG;
+  if (B > verify_max_requests() || V > (1 << 20)) return MA_ERR_UNSUPPORTED;
+  if (!workspace || workspace_bytes < ma_verify_drafts_workspace(B, V)) return MA_ERR_WORKSPACE;
+  VerifyParams p;
+  p.target = target;
+  p.draft = K > 0 ? draft : nullptr;
+  p.st[0] = st[0];
+  p.st[1] = st[1];
+  p.sd[0] = draft && K > 0 ? sd[0] : 0;
+  p.sd[1] = draft && K > 0 ? sd[1] : 0;
+  p.tokens = tokens;
+  p.counts = counts;
+  p.uniforms = uniforms;
+  p.B = B;
+  p.K = K;
+  p.V = V;
+  plan_verify(B, V, p.chunk, p.chunks);
+  p.accepted = accepted;
+  p.out = out;
+  char* base = align256(workspace) + 256;
+  p.tickets = reinterpret_cast<unsigned*>(base);
+  p.sums = reinterpret_cast<unsigned long long*>(base + kVerifyTickets * sizeof(unsigned));
+  return launch_verify_drafts(p, dtype, (cudaStream_t)stream);
+}
+
 }  // extern "C"

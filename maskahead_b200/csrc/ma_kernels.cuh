@@ -189,4 +189,70 @@ int launch_head_gather(const void* part, const int64_t sp[3], int B, int Hl, int
 // device properties, cached per device
 int device_sm_count();
 
+// ma_decode.cu: attention of few bf16 rows over a token-mode k4v4 cache read in place
+struct DecodeParams {
+  const __nv_bfloat16* q;
+  int64_t sq[3];
+  ma_kv kv;
+  ma_block cur;
+  int B, H, G, T, D, R;
+  float scale;
+  int causal;
+  __nv_bfloat16* out;
+  int64_t so[3];
+  unsigned* tickets;   // [B][H][row tiles], zero between calls
+  float2* ml;          // [H][row tiles][slots][rows] (m in log2 units, l) of every split
+  float* acc;          // [H][row tiles][slots][rows][D] their unnormalized outputs
+  int slots;           // splits per (head, row tile): the grid's x extent
+  int target;          // chunks the live slots are spread over
+  int min_units;       // shortest chunk, in 128-slot units
+  int row_tiles;
+};
+struct DecodePlan {
+  int rows, row_tiles, target, slots;
+};
+void plan_decode(int B, int H, int R, int Tc, DecodePlan& plan);
+int launch_decode_attention(DecodeParams& p, cudaStream_t st);
+
+// ma_pages.cu: page tables and slot maps from request lengths
+struct PagePlanParams {
+  const int32_t *lens, *new_lens, *pages, *free_list, *free_count;
+  int B, width, num_pages, page_size, max_tokens;
+  int64_t spg, spg_out;
+  int32_t *lens_out, *pages_out, *free_out, *count_out, *starts;
+  int64_t* slots;
+  int32_t *seqs, *positions;
+  unsigned* ticket;
+  int pages_in_place, free_in_place;
+};
+int page_plan_max_requests();
+int launch_page_plan(const PagePlanParams& p, cudaStream_t st);
+
+// ma_append.cu: K/V rows of new tokens quantized into the slots of a packed pool
+struct AppendParams {
+  const void *k, *v;
+  int64_t sk[2], sv[2];   // over (token, head)
+  int N, B, H, D;
+  const int64_t* slots;
+  const int32_t* seqs;
+  ma_kv kv;               // the pool (page_size, num_pages; strides over page, head, position)
+  void *k_rows, *v_rows;  // [N, H, D] the values the pool now holds, or null
+};
+int launch_append_tokens(const AppendParams& p, int dtype, cudaStream_t st);
+
+// ma_verify.cu: drafted tokens against the target's probabilities
+struct VerifyParams {
+  const void *target, *draft;   // [B, K + 1, V], [B, K, V] (draft null: one-hot drafts)
+  int64_t st[2], sd[2];         // strides over (request, position)
+  const int32_t *tokens, *counts;
+  const float* uniforms;        // [B, K + 1]
+  int B, K, V, chunk, chunks;
+  int32_t *accepted, *out;      // [B], [B, K + 1]
+  unsigned* tickets;            // [B], zero between calls
+  unsigned long long* sums;     // [B][chunks]
+};
+void plan_verify(int B, int V, int& chunk, int& chunks);
+int verify_max_requests();
+int launch_verify_drafts(const VerifyParams& p, int dtype, cudaStream_t st);
+
 }  // namespace ma

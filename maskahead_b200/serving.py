@@ -1,0 +1,379 @@
+"""One decoding step of a serving loop over a paged k4v4 cache.
+
+The select + attend path (hotpath.py) reads a paged cache; this module keeps one. Per step
+and layer a serving program
+
+  1. plans the step's slots from the requests' lengths (TokenPlan.build: page tables, free
+     stack, slot map, all on the device),
+  2. attends with few rows -- one token, or a short draft whose rows see each other causally --
+     over the packed pool read in place (PagedCache.attend, decode_attention),
+  3. verifies drafted tokens against the target's probabilities (verify_drafts),
+  4. appends the kept tokens' K/V rows through the slot map (PagedCache.append).
+
+The reference has no counterpart (its cache is contiguous, its sessions run one batch);
+the pool's arrays are its token-mode k4v4 layout (cache.py:142-189) with the page as the
+first axis. Everything runs on the current stream of the pool's device without waiting for
+it, and can be captured in a CUDA graph (run once before the capture, so that the shared
+workspace exists). Calls share one workspace per device and purpose, like the other
+operators: calls that can overlap on the GPU pass their own (`workspace`, a zeroed uint8
+tensor of decode_workspace_bytes / verify_workspace_bytes / PLAN_WORKSPACE_BYTES).
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from ._lib import MaBlock, MaRows, i64
+from .kernels._common import block_struct, rows_struct
+from .layouts import Prefix, as_prefix, kv_descriptor
+
+__all__ = ["PagedCache", "TokenPlan", "decode_attention", "verify_drafts", "decode_workspace_bytes",
+           "verify_workspace_bytes", "PLAN_WORKSPACE_BYTES", "MAX_DECODE_ROWS"]
+
+PLAN_WORKSPACE_BYTES = 512
+
+# Rows per KV head (query heads of the group x tokens) up to which attention reads the packed
+# cache in place; beyond, a prefix is unpacked once and the 128-row tensor-core tiles run.
+MAX_DECODE_ROWS = 64
+
+_GROUP = 32
+
+
+def _workspace(device: torch.device, purpose: str, nbytes: int, given: torch.Tensor | None) -> torch.Tensor:
+    if given is None:
+        return _lib.workspace(device, purpose, nbytes)
+    if given.dtype != torch.uint8 or not given.is_contiguous() or given.device != device or given.numel() < nbytes:
+        raise ValueError(f"workspace: need a contiguous uint8 tensor of at least {nbytes} bytes on {device}")
+    return given
+
+
+def decode_workspace_bytes(batch: int, heads: int, rows: int, head_dim: int, block_tokens: int = 0) -> int:
+    """Workspace of decode_attention: rows = query heads per KV head x tokens."""
+    return int(_lib.load_library().ma_decode_attention_workspace(batch, heads, rows, head_dim, block_tokens))
+
+
+def verify_workspace_bytes(batch: int, vocab: int) -> int:
+    return int(_lib.load_library().ma_verify_drafts_workspace(batch, vocab))
+
+
+def _check(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple, device: torch.device) -> None:
+    if t.dtype != dtype or tuple(t.shape) != shape or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape} on {device}, "
+                         f"got {t.dtype} {tuple(t.shape)} on {t.device}")
+
+
+# --------------------------------------------------------------------------- slot planning
+class TokenPlan:
+    """The slots of a step's new tokens, planned on the device from the requests' lengths.
+
+    lens [B] int32 and pages [B, width] int32 describe the requests now (request b holds
+    ceil(lens[b] / page_size) pages), free [num_pages] int32 is a stack of free_count [1]
+    unused pages. build(new_lens) plans the step: shorter requests hand pages back, longer
+    ones take pages from the stack in request order while pages and max_tokens last (from the
+    first that does not fit on, none grows: lens then differs from new_lens there).
+
+    After build the attributes hold: lens, pages, free, free_count (the new state; the tensors
+    given when in_place, else tensors of the plan's own), starts [B + 1] int32, and per new
+    token slots [max_tokens] int64 (page * page_size + offset), seqs and positions
+    [max_tokens] int32, -1 past the last token. They are the plan's buffers: the next build
+    overwrites them.
+    """
+
+    def __init__(self, *, lens: torch.Tensor, pages: torch.Tensor, free: torch.Tensor, free_count: torch.Tensor,
+                 page_size: int, num_pages: int, max_tokens: int, in_place: bool = True):
+        dev = lens.device
+        if dev.type != "cuda":
+            raise _lib.KernelUnavailableError("maskahead_b200 kernels need CUDA tensors")
+        if lens.ndim != 1 or pages.ndim != 2 or pages.shape[0] != lens.shape[0]:
+            raise ValueError("lens must be [B] and pages [B, width]")
+        b, width = pages.shape
+        if pages.dtype != torch.int32 or pages.device != dev or (pages.stride(1) != 1 and width > 1):
+            raise ValueError(f"pages must be int32 on {dev} with a contiguous page axis")
+        _check("lens", lens, torch.int32, (b,), dev)
+        _check("free", free, torch.int32, (num_pages,), dev)
+        _check("free_count", free_count, torch.int32, (1,), dev)
+        if page_size <= 0 or max_tokens < 0 or b == 0:
+            raise ValueError("need at least one request, page_size > 0 and max_tokens >= 0")
+        self.device, self.batch, self.width = dev, b, width
+        self.page_size, self.num_pages, self.max_tokens = int(page_size), int(num_pages), int(max_tokens)
+        self._in = (lens, pages, free, free_count)
+        if in_place:
+            self.lens, self.pages, self.free, self.free_count = self._in
+        else:
+            self.lens, self.free = torch.empty_like(lens), torch.empty_like(free)
+            self.pages = torch.empty((b, width), device=dev, dtype=torch.int32)
+            self.free_count = torch.empty_like(free_count)
+        self.starts = torch.empty(b + 1, device=dev, dtype=torch.int32)
+        self.slots = torch.empty(max_tokens, device=dev, dtype=torch.int64)
+        self.seqs = torch.empty(max_tokens, device=dev, dtype=torch.int32)
+        self.positions = torch.empty(max_tokens, device=dev, dtype=torch.int32)
+        self._call = _lib.lib().ma_page_plan
+        self._a = (b, pages.data_ptr(), pages.stride(0) if b > 1 else width, width, free.data_ptr(),
+                   free_count.data_ptr(), self.num_pages, self.page_size, self.max_tokens, self.lens.data_ptr(),
+                   self.pages.data_ptr(), self.pages.stride(0) if b > 1 else width, self.free.data_ptr(),
+                   self.free_count.data_ptr(), self.starts.data_ptr(), self.slots.data_ptr(), self.seqs.data_ptr(),
+                   self.positions.data_ptr())
+
+    def build(self, new_lens: torch.Tensor, *, workspace: torch.Tensor | None = None) -> "TokenPlan":
+        """Plan the step whose requests shall have new_lens [B] int32 tokens; returns self."""
+        _check("new_lens", new_lens, torch.int32, (self.batch,), self.device)
+        ws = _workspace(self.device, "page_plan", PLAN_WORKSPACE_BYTES, workspace)
+        rc = self._call(self._in[0].data_ptr(), new_lens.data_ptr(), *self._a, ws.data_ptr(), ws.numel(),
+                        _lib.stream_handle(self.device))
+        if rc:
+            _lib.check("ma_page_plan", rc)
+        return self
+
+
+# ----------------------------------------------------------------------------- the cache
+class PagedCache:
+    """A pool of token-mode k4v4 pages with its requests' tables.
+
+    kq, vq [P, H, page_size, D/32, 16] uint8 codes, ks, kz, vs, vz [P, H, page_size, D/32]
+    float16, kchan [B, H, D] float32 key divisors, pages [B, max_pages] int32, lens [B]
+    int32; free [P] int32 and free_count [1] int32 (optional) the stack of unused pages. The
+    cache addresses these tensors for its life; lens and pages are read on the device by
+    every call.
+    """
+
+    def __init__(self, *, kq, ks, kz, vq, vs, vz, kchan, pages, lens, free=None, free_count=None):
+        self.kq, self.ks, self.kz, self.vq, self.vs, self.vz = kq, ks, kz, vq, vs, vz
+        self.kchan, self.pages, self.lens, self.free, self.free_count = kchan, pages, lens, free, free_count
+        if kq.ndim != 5 or not kq.is_cuda:
+            raise ValueError("kq must be a rank-5 CUDA tensor [P, H, page_size, D/32, 16]")
+        self.num_pages, self.heads, self.page_size = kq.shape[0], kq.shape[1], kq.shape[2]
+        self.head_dim = kq.shape[3] * _GROUP
+        for name, t in (("ks", ks), ("kz", kz), ("vs", vs), ("vz", vz)):
+            if tuple(t.shape) != tuple(kq.shape[:4]):
+                raise ValueError(f"{name} must be [P, H, page_size, D/32] = {tuple(kq.shape[:4])}")
+        if tuple(vq.shape) != tuple(kq.shape) or kq.shape[4] != _GROUP // 2:
+            raise ValueError("kq and vq must be [P, H, page_size, D/32, 16]")
+        self.batch = pages.shape[0]
+        if tuple(kchan.shape) != (self.batch, self.heads, self.head_dim):
+            raise ValueError(f"kchan must be [B, H, D] = {(self.batch, self.heads, self.head_dim)}")
+        self.device = kq.device
+        for t in (ks, kz, vq, vs, vz, kchan, pages, lens):
+            if t.device != self.device:
+                raise ValueError("a cache's tensors must lie on one device")
+        self._desc = kv_descriptor(self.prefix())       # checks types and strides
+        self._lib = _lib.lib()
+        self._bytes: dict[tuple, int] = {}
+
+    @classmethod
+    def allocate(cls, *, batch: int, heads: int, head_dim: int, num_pages: int, page_size: int, max_pages: int,
+                 kchan: torch.Tensor, device="cuda") -> "PagedCache":
+        """An empty cache: every page on the free stack, every request of length 0."""
+        groups = head_dim // _GROUP
+        q = [torch.zeros((num_pages, heads, page_size, groups, _GROUP // 2), device=device, dtype=torch.uint8)
+             for _ in range(2)]
+        s = [torch.zeros((num_pages, heads, page_size, groups), device=device, dtype=torch.float16) for _ in range(4)]
+        return cls(kq=q[0], ks=s[0], kz=s[1], vq=q[1], vs=s[2], vz=s[3], kchan=kchan,
+                   pages=torch.full((batch, max_pages), -1, device=device, dtype=torch.int32),
+                   lens=torch.zeros(batch, device=device, dtype=torch.int32),
+                   free=torch.arange(num_pages - 1, -1, -1, device=device, dtype=torch.int32),
+                   free_count=torch.full((1,), num_pages, device=device, dtype=torch.int32))
+
+    def prefix(self) -> Prefix:
+        """The cache as the prefix of the other operators (every live slot)."""
+        return Prefix(kq=self.kq, ks=self.ks, kz=self.kz, vq=self.vq, vs=self.vs, vz=self.vz,
+                      nq=self.pages.shape[1] * self.page_size, kb=4, vb=4, kg=_GROUP, vg=_GROUP, kmode=1,
+                      kch=self.kchan, pages=self.pages, page_size=self.page_size, lens=self.lens)
+
+    def plan(self, max_tokens: int) -> TokenPlan:
+        """A TokenPlan over this cache's tables, updated in place by its build."""
+        if self.free is None or self.free_count is None:
+            raise ValueError("the cache was made without its free stack (free, free_count)")
+        return TokenPlan(lens=self.lens, pages=self.pages, free=self.free, free_count=self.free_count,
+                         page_size=self.page_size, num_pages=self.num_pages, max_tokens=max_tokens)
+
+    def append(self, key: torch.Tensor, value: torch.Tensor, slots: torch.Tensor, seqs: torch.Tensor, *,
+               return_rows: bool = False):
+        """Quantize the tokens' K/V rows [N, H, D] (bfloat16 or float32) into the pool: token i
+        into slots[i] (int64, as TokenPlan gives them; outside the pool: not stored), its keys
+        divided by the divisor of request seqs[i] (int32). The bytes are those of
+        layouts.quantize_tokens. return_rows: also the values the slots now stand for, (k, v)
+        [N, H, D] in the rows' type."""
+        if key.ndim != 3 or key.shape != value.shape or key.dtype != value.dtype:
+            raise ValueError("key and value must be [N, H, D] tensors of one shape and type")
+        n = key.shape[0]
+        if tuple(key.shape[1:]) != (self.heads, self.head_dim):
+            raise ValueError(f"rows must be [N, {self.heads}, {self.head_dim}]")
+        if key.device != self.device or value.device != self.device:
+            raise ValueError(f"rows must lie on {self.device}")
+        _check("slots", slots, torch.int64, (n,), self.device)
+        _check("seqs", seqs, torch.int32, (n,), self.device)
+        code = _lib.dtype_code(key.dtype)
+        k, v = _rows3(key), _rows3(value)
+        rows_k = rows_v = None
+        if return_rows:
+            rows_k = torch.empty((n, self.heads, self.head_dim), device=self.device, dtype=key.dtype)
+            rows_v = torch.empty_like(rows_k)
+        rc = self._lib.ma_append_tokens(
+            self._desc.kv, self.batch, self.heads, self.head_dim, k.data_ptr(), v.data_ptr(), code, n,
+            i64(*k.stride()[:2]), i64(*v.stride()[:2]), slots.data_ptr(), seqs.data_ptr(), _lib.ptr(rows_k),
+            _lib.ptr(rows_v), _lib.stream_handle(self.device))
+        if rc:
+            _lib.check("ma_append_tokens", rc)
+        return (rows_k, rows_v) if return_rows else None
+
+    def attend(self, query: torch.Tensor, current_key: torch.Tensor | None = None,
+               current_value: torch.Tensor | None = None, *, scaling: float | None = None, causal: bool = True,
+               out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
+        """decode_attention over this cache."""
+        return _attend(query, self, self._desc, current_key, current_value, scaling, causal, out, workspace)
+
+
+def _rows3(t: torch.Tensor) -> torch.Tensor:
+    """[N, H, D] rows with a contiguous, 16-byte aligned last axis, copying if not."""
+    es = t.element_size()
+    ok = t.stride(2) == 1 and t.data_ptr() % 16 == 0 and (t.stride(0) * es) % 16 == 0 and (t.stride(1) * es) % 16 == 0
+    return t if ok else t.contiguous()
+
+
+# ----------------------------------------------------------------------------- attention
+def decode_attention(query: torch.Tensor, prefix, current_key: torch.Tensor | None = None,
+                     current_value: torch.Tensor | None = None, *, scaling: float | None = None, causal: bool = True,
+                     out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of a few rows per request, query [B, Hq, T, D], over [live prefix | the step's
+    own keys current_key / current_value [B, Hkv, Tc, D]]; returns [B, Hq, T, D].
+
+    causal: row t sees the step's key j iff j <= t + Tc - T (Tc >= T; a draft's tokens see the
+    ones before them), else all of them. prefix: a PagedCache, a Prefix or a cache view.
+    Token-mode k4v4 storage without a dense tail (contiguous or paged, ragged, masked) is read
+    in place when the query is bfloat16 and a KV head has at most MAX_DECODE_ROWS rows; its
+    elements are then not rounded to bfloat16. Everything else runs as splitk_attention,
+    over a bfloat16 copy of a packed prefix. A row that sees no key is zero.
+    """
+    if isinstance(prefix, PagedCache):
+        return _attend(query, prefix, prefix._desc, current_key, current_value, scaling, causal, out, workspace)
+    pre = as_prefix(prefix)
+    return _attend(query, pre, None, current_key, current_value, scaling, causal, out, workspace)
+
+
+def _attend(query, source, desc, current_key, current_value, scaling, causal, out, workspace):
+    if query.ndim != 4:
+        raise ValueError("query must have shape [B, Hq, T, D]")
+    b, hq, t, d = query.shape
+    tc = 0 if current_key is None else current_key.shape[2]
+    if current_key is not None and (current_value is None or current_key.shape != current_value.shape
+                                    or current_key.ndim != 4):
+        raise ValueError("current K and V must be [B, Hkv, Tc, D] tensors of one shape")
+    if causal and 0 < tc < t:
+        raise ValueError(f"causal rows need at least as many current keys as rows: Tc={tc} < T={t}")
+    cached = isinstance(source, PagedCache)
+    if cached:
+        heads = source.heads
+        if b != source.batch or d != source.head_dim:
+            raise ValueError(f"query must be [{source.batch}, Hq, T, {source.head_dim}]")
+    else:
+        stored = source.kf if source.kf is not None else source.vq
+        if stored is None and current_key is None:
+            raise ValueError("nothing to attend: an empty prefix and no current keys")
+        heads = current_key.shape[1] if stored is None else stored.shape[1]
+    if hq % heads:
+        raise ValueError("Hq must be divisible by Hkv")
+    if current_key is not None and (current_key.shape[0] != b or current_key.shape[1] != heads
+                                    or current_key.shape[3] != d):
+        raise ValueError(f"current K and V must be [{b}, {heads}, Tc, {d}]")
+    rows = hq // heads * t
+    if out is not None and (out.shape != query.shape or out.dtype != query.dtype or out.device != query.device
+                            or out.stride(-1) != 1):
+        raise ValueError("out must match the query's shape, type and device, with a contiguous head_dim")
+    lib = _lib.lib()
+    if query.dtype == torch.bfloat16 and rows <= MAX_DECODE_ROWS and (
+            cached or (source.nq > 0 and source.nf == 0 and source.kmode == 1)):
+        if desc is None:
+            desc = kv_descriptor(source, batch=b, heads=heads, head_dim=d)
+        r, q = _rows(query)
+        blk, keep = _block(current_key, current_value)
+        o = torch.empty((b, hq, t, d), device=query.device, dtype=query.dtype) if out is None else out
+        key = (b, heads, rows, d, tc)
+        nbytes = source._bytes.get(key) if cached else None
+        if nbytes is None:
+            nbytes = lib.ma_decode_attention_workspace(*key)
+            if cached:
+                source._bytes[key] = nbytes
+        ws = _workspace(query.device, "decode", nbytes, workspace)
+        rc = lib.ma_decode_attention(r, desc.kv, heads, blk, d ** -0.5 if scaling is None else float(scaling),
+                                     1 if causal else 0, o.data_ptr(), i64(*o.stride()[:3]), ws.data_ptr(), ws.numel(),
+                                     _lib.stream_handle(query.device))
+        if rc == _lib.MA_OK:
+            return o
+        if rc != _lib.MA_ERR_UNSUPPORTED:
+            _lib.check("ma_decode_attention", rc)
+        del q, keep
+    return _attend_general(query, source, current_key, current_value, scaling, causal, out)
+
+
+def _rows(query: torch.Tensor):
+    return rows_struct(query)
+
+
+def _block(key, value):
+    return block_struct(key, value, torch.bfloat16)
+
+
+def _attend_general(query, source, current_key, current_value, scaling, causal, out):
+    from .hotpath import unpacked_prefix
+    from .kernels.splitk import splitk_attention
+
+    prefix = source.prefix() if isinstance(source, PagedCache) else source
+    b, hq, t, d = query.shape
+    if query.dtype == torch.bfloat16 and prefix.nq > 0:
+        prefix = unpacked_prefix(prefix, b, prefix.vq.shape[1], d)
+    tc = 0 if current_key is None else current_key.shape[2]
+    res, _ = splitk_attention(query, prefix, current_key, current_value, scaling=scaling,
+                              causal_block=1 if causal and tc else 0, q_pos0=tc - t, c_pos0=0)
+    if out is None:
+        return res
+    out.copy_(res)
+    return out
+
+
+# -------------------------------------------------------------------------- verification
+def verify_drafts(target: torch.Tensor, draft: torch.Tensor | None, tokens: torch.Tensor,
+                  counts: torch.Tensor | None, uniforms: torch.Tensor, *, workspace: torch.Tensor | None = None):
+    """Accept or refuse drafted tokens against the target's probabilities and draw the next.
+
+    target [B, K + 1, V] (float32, bfloat16 or float16): the target's probabilities after the
+    context and after each draft; draft [B, K, V] of the same type: the distributions the
+    drafts were drawn from (None: each draft was certain, e.g. greedy or looked up); tokens
+    [B, K] int32; counts [B] int32 drafts in use (None: K); uniforms [B, K + 1] float32 in
+    [0, 1). Draft i is accepted while u_i q_i(x_i) < p_i(x_i); after a accepted drafts the next
+    token is drawn from max(p_a - q_a, 0), or from p_a when all were accepted, with the last
+    uniform: every emitted token is then distributed as the target's own. The drawing sums
+    whole numbers (floor(r 2^40)), so the same inputs give the same token on any GPU.
+
+    Returns (accepted [B] int32, tokens [B, K + 1] int32: the accepted drafts, the next token,
+    then -1); tokens[b, accepted[b]] is -1 only when p_a has no mass.
+    """
+    if target.ndim != 3 or target.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise ValueError("target must be a float32, bfloat16 or float16 tensor [B, K + 1, V]")
+    b, k1, v = target.shape
+    k, dev = k1 - 1, target.device
+    if dev.type != "cuda":
+        raise _lib.KernelUnavailableError("maskahead_b200 kernels need CUDA tensors")
+    if k < 0 or b == 0 or v == 0:
+        raise ValueError("target must be [B, K + 1, V] with B, V >= 1 and K >= 0")
+    if target.stride(2) != 1 and v > 1:
+        raise ValueError("target must have a contiguous vocabulary axis")
+    if draft is not None and (draft.dtype != target.dtype or tuple(draft.shape) != (b, k, v) or draft.device != dev
+                              or (draft.stride(2) != 1 and v > 1)):
+        raise ValueError(f"draft must be a {target.dtype} tensor {(b, k, v)} on {dev} with a contiguous vocabulary axis")
+    _check("tokens", tokens, torch.int32, (b, k), dev)
+    _check("uniforms", uniforms, torch.float32, (b, k1), dev)
+    if counts is not None:
+        _check("counts", counts, torch.int32, (b,), dev)
+    lib = _lib.lib()
+    accepted = torch.empty(b, device=dev, dtype=torch.int32)
+    out = torch.empty((b, k1), device=dev, dtype=torch.int32)
+    ws = _workspace(dev, "verify", lib.ma_verify_drafts_workspace(b, v), workspace)
+    code = _lib.MA_F16 if target.dtype == torch.float16 else _lib.dtype_code(target.dtype)
+    rc = lib.ma_verify_drafts(target.data_ptr(), _lib.ptr(draft), code, b, k, v, i64(target.stride(0), target.stride(1)),
+                              i64(draft.stride(0), draft.stride(1)) if draft is not None else None,
+                              tokens.data_ptr(), _lib.ptr(counts), uniforms.data_ptr(), accepted.data_ptr(),
+                              out.data_ptr(), ws.data_ptr(), ws.numel(), _lib.stream_handle(dev))
+    if rc:
+        _lib.check("ma_verify_drafts", rc)
+    return accepted, out
