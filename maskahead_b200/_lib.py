@@ -159,11 +159,18 @@ def load_library() -> ctypes.CDLL:
     return lib
 
 
+_ready: ctypes.CDLL | None = None
+
+
 def lib() -> ctypes.CDLL:
-    """The library, for a compute call: also requires a CUDA device."""
-    if not torch.cuda.is_available():
-        raise KernelUnavailableError("maskahead_b200 kernels need a CUDA device (sm_100a)")
-    return load_library()
+    """The library, for a compute call: also requires a CUDA device (looked for once: a
+    process's devices do not go away, and the look costs 3 us)."""
+    global _ready
+    if _ready is None:
+        if not torch.cuda.is_available():
+            raise KernelUnavailableError("maskahead_b200 kernels need a CUDA device (sm_100a)")
+        _ready = load_library()
+    return _ready
 
 
 def check(fn: str, status: int) -> None:
@@ -191,7 +198,14 @@ def i64(*vals) -> ctypes.Array:
     return (ctypes.c_int64 * len(vals))(*[int(v) for v in vals])
 
 
+# The current stream's handle without building a torch.cuda.Stream object (1.5 us a call), as
+# torch's own generated code takes it; the public way where a torch lacks it.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_handle(device: torch.device) -> int:
+    if _raw_stream is not None and device.index is not None:
+        return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
 

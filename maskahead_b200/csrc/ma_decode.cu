@@ -27,10 +27,9 @@ namespace ma {
 
 namespace {
 
-constexpr int kWarps = 4;
 constexpr int kTile = 32;                 // slots per warp tile
-constexpr int kUnit = kWarps * kTile;     // chunk granularity in slots
-constexpr int kStages = 3;
+constexpr int kUnit = 256;                // chunk granularity in slots
+constexpr int kStages = 2;
 constexpr float kLog2e = 1.4426950408889634f;
 
 // Shared memory of one ring stage: K payload, V payload (D/2 bytes a slot each), then the
@@ -42,6 +41,7 @@ struct Ring {
   static constexpr int kVq = kPay, kKs = 2 * kPay, kKz = kKs + kSc, kVs = kKz + kSc, kVz = kVs + kSc;
   static constexpr int kStage = kVz + kSc;
   static constexpr int kWarpBytes = kStages * kStage;
+  static_assert(kStage % 128 == 0, "stages keep the swizzle's 128-byte phase");
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
@@ -78,8 +78,15 @@ __device__ __forceinline__ void mma16(float c[4], uint32_t a0, uint32_t a1, uint
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void mma8(float c[4], uint32_t a0, uint32_t a1, uint32_t b0) {
-  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};\n"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(b0));
+  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%7,%7,%7,%7};\n"
+               : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(b0), "f"(0.f));
+}
+// the first product of a sum: c = a b
+__device__ __forceinline__ void mma16_set(float c[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                          uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+               : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -195,82 +202,13 @@ __device__ __forceinline__ void store_row4(const DecodeParams& p, int b, int h, 
   store4(dst, o.x, o.y, o.z, o.w);
 }
 
-// Merge of the partials of one (b, h, row tile) by a whole CTA: warp w takes splits w, w + 4,
-// ..., then the warps' sums meet in shared memory. sW: [kWarps][kPad] floats per row pass.
-template <int D, int ROWS>
-__device__ void merge_partials(const DecodeParams& p, const Split& s, int b, int h, int bhr, int r0, int rows,
-                               float* sAcc) {
-  constexpr int kVec = D / 4, kPad = D + 4, kGroups = kWarps * 32 / kVec;   // thread groups of one row each
-  __shared__ float sML[ROWS * 2];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const float2* ml = p.ml + (int64_t)bhr * p.slots * ROWS;
-  const float* acc = p.acc + (int64_t)bhr * p.slots * ROWS * D;
-  const int chunks = p.cur.Tc > 0 ? s.count - 1 : s.count;
-  auto place = [&](int i) { return i < chunks ? s.first + i : s.total + b; };
-  // per row the maximum over the splits and the sum of the rescaled l
-  for (int r = warp; r < rows; r += kWarps) {
-    float m = -INFINITY;
-    for (int i = lane; i < s.count; i += 32) m = fmaxf(m, __ldcg(&ml[(int64_t)place(i) * ROWS + r]).x);
-    m = warp_max(m);
-    const float ms = m == -INFINITY ? 0.f : m;
-    float l = 0.f;
-    for (int i = lane; i < s.count; i += 32) {
-      const float2 v = __ldcg(&ml[(int64_t)place(i) * ROWS + r]);
-      l += v.y * ex2(v.x - ms);
-    }
-    l = warp_sum(l);
-    if (lane == 0) {
-      sML[2 * r] = ms;
-      sML[2 * r + 1] = l;
-    }
-  }
-  __syncthreads();
-  const int grp = tid / kVec, d = (tid % kVec) * 4;
-  for (int r = 0; r < rows; ++r) {
-    const float ms = sML[2 * r];
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int i = grp; i < s.count; i += kGroups) {
-      const int64_t at = (int64_t)place(i) * ROWS + r;
-      const float w = ex2(__ldcg(&ml[at]).x - ms);
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(acc + at * D + d));
-      o.x = fmaf(w, v.x, o.x);
-      o.y = fmaf(w, v.y, o.y);
-      o.z = fmaf(w, v.z, o.z);
-      o.w = fmaf(w, v.w, o.w);
-    }
-    *reinterpret_cast<float4*>(sAcc + (r * kGroups + grp) * kPad + d) = o;
-  }
-  __syncthreads();
-  for (int i = tid; i < rows * kVec; i += kWarps * 32) {
-    const int r = i / kVec, dd = (i % kVec) * 4;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int g = 0; g < kGroups; ++g) {
-      const float4 v = *reinterpret_cast<const float4*>(sAcc + (r * kGroups + g) * kPad + dd);
-      o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
-    }
-    const float l = sML[2 * r + 1];
-    const float inv = l > 0.f ? 1.f / l : 0.f;
-    store_row4<D>(p, b, h, r0 + r, dd, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
-  }
-}
-
 // A CTA's result from nsrc sources in shared memory -- sRows[nsrc][ROWS][kPad] unnormalized
-// rows, sML[nsrc][ROWS] their (m, l): the output rows when it is the sequence's only split,
-// else this split's partial and, in the last CTA to arrive, the merge of all of them.
-template <int D, int ROWS>
-__device__ void finish(const DecodeParams& p, const Split& s, int h, int rt, int slot, int nsrc, float* sRows,
-                       const float2* sML) {
+// rows, sML[nsrc][ROWS] their (m, l) -- to the output rows (normalized) or to partial `slot`.
+template <int D, int ROWS, int W>
+__device__ __forceinline__ void combine(const DecodeParams& p, int b, int h, int r0, int rows, int nsrc, const float* sRows,
+                                        const float2* sML, float2* ml, float* acc) {
   constexpr int kVec = D / 4, kPad = D + 4;
-  __shared__ int sLast;
-  const int tid = threadIdx.x;
-  const int r0 = rt * ROWS, rows = min(ROWS, p.R - r0);
-  const int b = s.b;
-  const int bhr = h * p.row_tiles + rt;
-  float2* ml = p.ml + (int64_t)bhr * p.slots * ROWS;
-  float* acc = p.acc + (int64_t)bhr * p.slots * ROWS * D;
-  for (int i = tid; i < rows * kVec; i += kWarps * 32) {
+  for (int i = threadIdx.x; i < rows * kVec; i += W * 32) {
     const int r = i / kVec, d = (i % kVec) * 4;
     float m = -INFINITY;
     for (int w = 0; w < nsrc; ++w) m = fmaxf(m, sML[w * ROWS + r].x);
@@ -287,19 +225,95 @@ __device__ void finish(const DecodeParams& p, const Split& s, int h, int rt, int
       o.z = fmaf(f, v.z, o.z);
       o.w = fmaf(f, v.w, o.w);
     }
-    if (s.count == 1) {
+    if (acc == nullptr) {
       const float inv = l > 0.f ? 1.f / l : 0.f;
       store_row4<D>(p, b, h, r0 + r, d, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
     } else {
-      const int64_t at = (int64_t)slot * ROWS + r;
-      __stcg(reinterpret_cast<float4*>(acc + at * D + d), o);
-      if (d == 0) __stcg(&ml[at], make_float2(m, l));
+      __stcg(reinterpret_cast<float4*>(acc + r * D + d), o);
+      if (d == 0) __stcg(&ml[r], make_float2(m, l));
     }
   }
-  if (s.count == 1) return;
+}
+
+// The merge of a sequence's partials, in the last of its CTAs: warp w folds splits w, w + W, ...
+// into running rows (8 rows at a time, two splits in flight), then the warps' rows are combined
+// as a CTA's own are. The order is fixed, so the result does not depend on who came last.
+template <int D, int ROWS, int W>
+__device__ void merge_partials(const DecodeParams& p, const Split& s, int b, int h, int r0, int rows, const float2* ml,
+                               const float* acc, float* sRows, float2* sML) {
+  constexpr int kPad = D + 4, kLanes = D / 4;         // lanes of a row; with 64 channels a warp reads two at once
+  constexpr int kPer = 32 / kLanes, kStep = 8 / kPer;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int chunks = p.cur.Tc > 0 ? s.count - 1 : s.count;
+  const int sub = lane / kLanes, d = (lane % kLanes) * 4;
+  for (int g0 = 0; g0 < rows; g0 += 8) {
+    float m = -INFINITY, l = 0.f;                     // of row g0 + lane (lanes 0 .. 7)
+    float4 o[kStep];
+#pragma unroll
+    for (int k = 0; k < kStep; ++k) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = warp; i < s.count; i += 2 * W) {
+      float2 e[2];
+      float4 v[2][kStep];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int x = i + u * W;
+        e[u] = make_float2(-INFINITY, 0.f);
+        if (x < s.count) {
+          const int64_t at = (int64_t)(x < chunks ? s.first + x : s.total + b) * ROWS + g0;
+          if (lane < 8 && g0 + lane < rows) e[u] = __ldcg(&ml[at + lane]);
+#pragma unroll
+          for (int k = 0; k < kStep; ++k) {
+            const int r = k * kPer + sub;
+            v[u][k] = g0 + r < rows ? __ldcg(reinterpret_cast<const float4*>(acc + (at + r) * D + d))
+                                    : make_float4(0.f, 0.f, 0.f, 0.f);
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        if (i + u * W >= s.count) break;
+        const float mn = fmaxf(m, e[u].x), ms = mn == -INFINITY ? 0.f : mn;
+        const float old = ex2(m - ms), add = ex2(e[u].x - ms);
+        m = mn;
+        l = l * old + e[u].y * add;
+#pragma unroll
+        for (int k = 0; k < kStep; ++k) {
+          const float f = __shfl_sync(0xffffffffu, old, k * kPer + sub), w = __shfl_sync(0xffffffffu, add, k * kPer + sub);
+          o[k].x = fmaf(w, v[u][k].x, o[k].x * f);
+          o[k].y = fmaf(w, v[u][k].y, o[k].y * f);
+          o[k].z = fmaf(w, v[u][k].z, o[k].z * f);
+          o[k].w = fmaf(w, v[u][k].w, o[k].w * f);
+        }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kStep; ++k)
+      *reinterpret_cast<float4*>(sRows + (warp * ROWS + g0 + k * kPer + sub) * kPad + d) = o[k];
+    if (lane < 8) sML[warp * ROWS + g0 + lane] = make_float2(m, l);
+  }
+  __syncthreads();
+  combine<D, ROWS, W>(p, b, h, r0, rows, W, sRows, sML, nullptr, nullptr);
+}
+
+// The CTA's rows: the output when they are the sequence's only split, else this split's partial
+// and, in the last CTA to arrive, the merge of all of them.
+template <int D, int ROWS, int W>
+__device__ void finish(const DecodeParams& p, const Split& s, int h, int rt, int slot, int nsrc, float* sRows, float2* sML,
+                       float2* sMerge) {
+  __shared__ int sLast;
+  const int r0 = rt * ROWS, rows = min(ROWS, p.R - r0);
+  const int b = s.b;
+  if (s.count == 1) {
+    combine<D, ROWS, W>(p, b, h, r0, rows, nsrc, sRows, sML, nullptr, nullptr);
+    return;
+  }
+  const int64_t base = (int64_t)(h * p.row_tiles + rt) * p.slots * ROWS;
+  float2* ml = p.ml + base;
+  float* acc = p.acc + base * D;
+  combine<D, ROWS, W>(p, b, h, r0, rows, nsrc, sRows, sML, ml + (int64_t)slot * ROWS, acc + (int64_t)slot * ROWS * D);
   __threadfence();
   __syncthreads();
-  if (tid == 0) {
+  if (threadIdx.x == 0) {
     unsigned* ticket = p.tickets + ((int64_t)b * p.H + h) * p.row_tiles + rt;
     const unsigned got = atomicAdd(ticket, 1u);
     sLast = got == (unsigned)s.count - 1u;
@@ -308,23 +322,23 @@ __device__ void finish(const DecodeParams& p, const Split& s, int h, int rt, int
   __syncthreads();
   if (!sLast) return;
   __threadfence();
-  merge_partials<D, ROWS>(p, s, b, h, bhr, r0, rows, sRows);
+  merge_partials<D, ROWS, W>(p, s, b, h, r0, rows, ml, acc, sRows, sMerge);
 }
 
 // The step's own keys: a warp per row, a lane per key, in fp32 (a few hundred products a row).
-template <int D, int ROWS>
+template <int D, int ROWS, int W>
 __device__ void block_split(const DecodeParams& p, const Split& s, int h, int rt, char* smem) {
   constexpr int kPad = D + 4;
   constexpr int kRow = D + 8;                              // staged bf16 row, 16 bytes of padding
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int b = s.b, r0 = rt * ROWS, rows = min(ROWS, p.R - r0);
-  float* sRows = reinterpret_cast<float*>(smem);            // [ROWS][kPad]: q first, the result later
-  __nv_bfloat16* sK = reinterpret_cast<__nv_bfloat16*>(smem + ROWS * kPad * 4);
+  float2* sML = reinterpret_cast<float2*>(smem);            // [W][ROWS]
+  float* sRows = reinterpret_cast<float*>(smem + W * ROWS * 8);     // [W][ROWS][kPad]: q first, the result later
+  __nv_bfloat16* sK = reinterpret_cast<__nv_bfloat16*>(smem + W * ROWS * 8 + ROWS * kPad * 4);
   __nv_bfloat16* sV = sK + 32 * kRow;
-  float2* sML = reinterpret_cast<float2*>(sV + 32 * kRow);
   const __nv_bfloat16* K = reinterpret_cast<const __nv_bfloat16*>(p.cur.k) + (int64_t)b * p.cur.sk[0] + (int64_t)h * p.cur.sk[1];
   const __nv_bfloat16* V = reinterpret_cast<const __nv_bfloat16*>(p.cur.v) + (int64_t)b * p.cur.sv[0] + (int64_t)h * p.cur.sv[1];
-  for (int i = tid; i < rows * (D / 8); i += kWarps * 32) {
+  for (int i = tid; i < rows * (D / 8); i += W * 32) {
     const int r = i / (D / 8), d = (i % (D / 8)) * 8;
     const int g = (r0 + r) / p.T, t = (r0 + r) - g * p.T;
     float f[8];
@@ -332,7 +346,7 @@ __device__ void block_split(const DecodeParams& p, const Split& s, int h, int rt
 #pragma unroll
     for (int e = 0; e < 8; ++e) sRows[r * kPad + d + e] = f[e];
   }
-  constexpr int kOwn = ROWS / kWarps;                       // rows per warp
+  constexpr int kOwn = (ROWS + W - 1) / W;                       // rows per warp
   constexpr int kCh = D / 32;                               // channels per lane
   float m[kOwn], l[kOwn], o[kOwn][kCh];
 #pragma unroll
@@ -345,7 +359,7 @@ __device__ void block_split(const DecodeParams& p, const Split& s, int h, int rt
   for (int j0 = 0; j0 < p.cur.Tc; j0 += 32) {
     const int nj = min(32, p.cur.Tc - j0);
     __syncthreads();
-    for (int i = tid; i < 32 * (D / 8); i += kWarps * 32) {
+    for (int i = tid; i < 32 * (D / 8); i += W * 32) {
       const int j = i / (D / 8), d = (i % (D / 8)) * 8;
       uint4 kv = make_uint4(0u, 0u, 0u, 0u), vv = kv;
       if (j < nj) {
@@ -358,7 +372,7 @@ __device__ void block_split(const DecodeParams& p, const Split& s, int h, int rt
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kOwn; ++i) {
-      const int r = warp + i * kWarps;
+      const int r = warp + i * W;
       if (r >= rows) break;
       const int t = (r0 + r) % p.T;
       const int seen = p.causal ? t + p.cur.Tc - p.T : p.cur.Tc - 1;    // the last key this row sees
@@ -392,19 +406,20 @@ __device__ void block_split(const DecodeParams& p, const Split& s, int h, int rt
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kOwn; ++i) {
-    const int r = warp + i * kWarps;
+    const int r = warp + i * W;
     if (r >= rows) break;
 #pragma unroll
     for (int c = 0; c < kCh; ++c) sRows[r * kPad + lane * kCh + c] = o[i][c];
     if (lane == 0) sML[r] = make_float2(m[i], l[i]);
   }
   __syncthreads();
-  finish<D, ROWS>(p, s, h, rt, s.total + b, 1, sRows, sML);
+  finish<D, ROWS, W>(p, s, h, rt, s.total + b, 1, sRows, sML, sML);
 }
 
-template <int D, int NT>
-__global__ void __launch_bounds__(kWarps * 32) decode_attention_kernel(const __grid_constant__ DecodeParams p) {
-  constexpr int ROWS = 8 * NT, NG = D / 32, kPad = D + 4;
+// FAST: tiles are contiguous in storage (launch() says when); else every slot is looked up alone.
+template <int D, int NT, int W, int MINB, bool FAST>
+__global__ void __launch_bounds__(W * 32, MINB) decode_attention_kernel(const __grid_constant__ DecodeParams p) {
+  constexpr int ROWS = 8 * NT, NG = D / 32, kPad = D + 4, kSc = D / 16;
   using R = Ring<D>;
   extern __shared__ __align__(128) char smem[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -414,7 +429,7 @@ __global__ void __launch_bounds__(kWarps * 32) decode_attention_kernel(const __g
   if (s.b < 0) return;
   const int b = s.b;
   if (s.chunk < 0) {
-    block_split<D, ROWS>(p, s, h, rt, smem);
+    block_split<D, ROWS, W>(p, s, h, rt, smem);
     return;
   }
   const ma_kv& kv = p.kv;
@@ -423,45 +438,92 @@ __global__ void __launch_bounds__(kWarps * 32) decode_attention_kernel(const __g
   const int end = (int)min((int64_t)n, begin + (int64_t)s.per * kUnit);
   const uint32_t ring = smem_u32(smem) + warp * R::kWarpBytes;
 
-  // ---- the copies of one tile: lane l resolves slot l (page, mask), the pieces of a slot's
-  // payload row go by neighbouring lanes
+  // ---- the copies of a tile of 32 slots into a ring stage. `find` looks a tile up (a load from
+  // the page table, one tile ahead of its use), `issue` starts its copies and returns its live
+  // slots; dead ones are zero-filled, so nothing stored there is ever multiplied.
   const int tiles = end > begin ? (int)((end - begin + kTile - 1) / kTile) : 0;
-  const uint8_t* kq = kv.kq + (int64_t)h * kv.skq[1];
-  const uint8_t* vq = kv.vq + (int64_t)h * kv.svq[1];
-  const uint16_t* ks = kv.ks + (int64_t)h * kv.sks[1];
-  const uint16_t* kz = kv.kz + (int64_t)h * kv.sks[1];
-  const uint16_t* vs = kv.vs + (int64_t)h * kv.svs[1];
-  const uint16_t* vz = kv.vz + (int64_t)h * kv.svs[1];
-  auto resolve = [&](int i, int& sb, int& sj) {      // storage coordinates of this lane's slot, sb -1: dead
-    const int64_t j = begin + (int64_t)i * kTile + lane;
-    sb = -1;
-    sj = 0;
-    if (i >= tiles || j >= end) return;
-    kv_page(kv, b, (int)j, sb, sj);
-    if (kv.mask != nullptr && kv.mask[((int64_t)b * p.H + h) * kv.nq + j] == 0) sb = -1;
+  constexpr int kPieces = D / 32, kSlots = 32 / kPieces;       // 16-byte pieces per slot, slots per pass
+  struct Place {
+    int page, at;      // FAST: of the tile, else of this lane's slot; page -1: dead
   };
-  auto issue = [&](int i, int stage, int sb, int sj) -> unsigned {
-    const bool live = sb >= 0;
-    const unsigned alive = __ballot_sync(0xffffffffu, live);
-    if (i < tiles) {
-      const uint32_t st = ring + stage * R::kStage;
-      const int64_t pb = live ? sb : 0, pj = live ? sj : 0;
-      const int64_t okq = pb * kv.skq[0] + pj * kv.skq[2], ovq = pb * kv.svq[0] + pj * kv.svq[2];
-      const int64_t oks = pb * kv.sks[0] + pj * kv.sks[2], ovs = pb * kv.svs[0] + pj * kv.svs[2];
-      constexpr int kSc = D / 16;
-      const uint32_t sc = live ? kSc : 0;
-      cp_async<kSc>(st + R::kKs + lane * kSc, ks + oks, sc);
-      cp_async<kSc>(st + R::kKz + lane * kSc, kz + oks, sc);
-      cp_async<kSc>(st + R::kVs + lane * kSc, vs + ovs, sc);
-      cp_async<kSc>(st + R::kVz + lane * kSc, vz + ovs, sc);
-      constexpr int kPieces = D / 32, kSlots = 32 / kPieces;     // pieces per slot, slots per pass
+  const int64_t hq = (int64_t)h * kv.skq[1], hs = (int64_t)h * kv.sks[1], hvq = (int64_t)h * kv.svq[1], hvs = (int64_t)h * kv.svs[1];
+  auto find = [&](int i) -> Place {
+    Place f = {-1, 0};
+    if constexpr (FAST) {
+      if (i < tiles) {
+        const int x = (int)(begin / kTile) + i;
+        f.page = b;
+        f.at = x;
+        if (kv.pages != nullptr) {
+          const int pi = p.tile_div.div(x);
+          f.at = x - pi * p.tiles_per_page;
+          f.page = kv.pages[(int64_t)b * kv.spg + pi];
+          if ((unsigned)f.page >= (unsigned)kv.num_pages) f.page = -1;
+        }
+      }
+    } else {
+      const int64_t j = begin + (int64_t)i * kTile + lane;
+      if (i < tiles && j < end) {
+        kv_page(kv, b, (int)j, f.page, f.at);
+        if (kv.mask != nullptr && kv.mask[((int64_t)b * p.H + h) * kv.nq + j] == 0) f.page = -1;
+      }
+    }
+    return f;
+  };
+  // FAST: this lane's share of a tile's contiguous 32 D/2 payload bytes and, in the order they
+  // have in a stage, of the four scale and zero blocks
+  constexpr int kScPieces = kTile * kSc / 16, kScLanes = kTile / kScPieces;    // 16-byte pieces per block, slots each
+  const char* lane_sc[NG / 2];
 #pragma unroll
-      for (int it = 0; it < kPieces; ++it) {
-        const int sl = it * kSlots + lane / kPieces, c = lane % kPieces;
-        const int64_t ok = __shfl_sync(0xffffffffu, okq, sl), ov = __shfl_sync(0xffffffffu, ovq, sl);
-        const uint32_t bytes = (alive >> sl & 1u) ? 16u : 0u;
-        cp_async<16>(st + piece<D>(sl, c), kq + ok + c * 16, bytes);
-        cp_async<16>(st + R::kVq + piece<D>(sl, c), vq + ov + c * 16, bytes);
+  for (int it = 0; it < NG / 2; ++it) {
+    const int blk = (it * 32 + lane) / kScPieces;
+    const uint16_t* base = blk == 0 ? kv.ks + hs : blk == 1 ? kv.kz + hs : blk == 2 ? kv.vs + hvs : kv.vz + hvs;
+    lane_sc[it] = reinterpret_cast<const char*>(base) + (lane % kScPieces) * 16;
+  }
+  const uint8_t* lane_kq = kv.kq + hq + (FAST ? lane * 16 : 0);
+  const uint8_t* lane_vq = kv.vq + hvq + (FAST ? lane * 16 : 0);
+  auto issue = [&](int i, int stage, Place f) -> unsigned {
+    unsigned alive;
+    const uint32_t st = ring + stage * R::kStage;
+    if constexpr (FAST) {
+      const int64_t left = end - (begin + (int64_t)i * kTile);
+      const int cnt = f.page < 0 ? 0 : (int)min((int64_t)kTile, left);
+      alive = cnt == kTile ? 0xffffffffu : (1u << cnt) - 1u;
+      if (i < tiles) {
+        const int64_t pg = max(f.page, 0);
+        const int64_t oq = pg * kv.skq[0] + (int64_t)f.at * (kTile * D / 2), os = (pg * kv.sks[0] + (int64_t)f.at * (kTile * NG)) * 2;
+#pragma unroll
+        for (int it = 0; it < kPieces; ++it) {
+          const int sl = it * kSlots + lane / kPieces, c = lane % kPieces;
+          const uint32_t bytes = sl < cnt ? 16u : 0u;
+          cp_async<16>(st + piece<D>(sl, c), lane_kq + oq + it * 512, bytes);
+          cp_async<16>(st + R::kVq + piece<D>(sl, c), lane_vq + oq + it * 512, bytes);
+        }
+        const int sc_left = (cnt - (lane % kScPieces) * kScLanes) * kSc;
+        const uint32_t bytes = min(max(sc_left, 0), 16);
+#pragma unroll
+        for (int it = 0; it < NG / 2; ++it) cp_async<16>(st + R::kKs + (it * 32 + lane) * 16, lane_sc[it] + os, bytes);
+      }
+    } else {
+      const bool live = f.page >= 0;
+      alive = __ballot_sync(0xffffffffu, live);
+      if (i < tiles) {
+        const int64_t pb = live ? f.page : 0, pj = live ? f.at : 0;
+        const int64_t okq = pb * kv.skq[0] + pj * kv.skq[2], ovq = pb * kv.svq[0] + pj * kv.svq[2];
+        const int64_t oks = hs + pb * kv.sks[0] + pj * kv.sks[2], ovs = hvs + pb * kv.svs[0] + pj * kv.svs[2];
+        const uint32_t sc = live ? kSc : 0;
+        cp_async<kSc>(st + R::kKs + lane * kSc, kv.ks + oks, sc);
+        cp_async<kSc>(st + R::kKz + lane * kSc, kv.kz + oks, sc);
+        cp_async<kSc>(st + R::kVs + lane * kSc, kv.vs + ovs, sc);
+        cp_async<kSc>(st + R::kVz + lane * kSc, kv.vz + ovs, sc);
+#pragma unroll
+        for (int it = 0; it < kPieces; ++it) {
+          const int sl = it * kSlots + lane / kPieces, c = lane % kPieces;
+          const int64_t ok = __shfl_sync(0xffffffffu, okq, sl), ov = __shfl_sync(0xffffffffu, ovq, sl);
+          const uint32_t bytes = (alive >> sl & 1u) ? 16u : 0u;
+          cp_async<16>(st + piece<D>(sl, c), lane_kq + ok + c * 16, bytes);
+          cp_async<16>(st + R::kVq + piece<D>(sl, c), lane_vq + ov + c * 16, bytes);
+        }
       }
     }
     cp_commit();
@@ -469,13 +531,9 @@ __global__ void __launch_bounds__(kWarps * 32) decode_attention_kernel(const __g
   };
 
   unsigned flight[kStages];        // live slots of the tiles in flight, the next tile's first
-  int sb, sj;
 #pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) {
-    resolve(warp + i * kWarps, sb, sj);
-    flight[i] = issue(warp + i * kWarps, i, sb, sj);
-  }
-  resolve(warp + (kStages - 1) * kWarps, sb, sj);
+  for (int i = 0; i < kStages - 1; ++i) flight[i] = issue(warp + i * W, i, find(warp + i * W));
+  Place next = find(warp + (kStages - 1) * W);
 
   // ---- the query rows as B operands: q' = q kchan in fp16, scaled by a power of two so that a
   // row's largest magnitude lies in [2^13, 2^14) (11 bits of q', where a bf16 cache would
@@ -483,7 +541,8 @@ __global__ void __launch_bounds__(kWarps * 32) decode_attention_kernel(const __g
   // channels (0, 4), (1, 5), (2, 6), (3, 7) of a word as its masks leave them, the odd ones with
   // q' / 16 because a high nibble is worth 16 times a low one.
   uint32_t qb[NT][NG][4], zb[NT];
-  float fr[NT][2];
+  float fr[NT][2];                 // score in log2 units = fr * sum, fr > 0: the scale's sign goes into q'
+  const float sign = p.scale > 0.f ? 1.f : p.scale < 0.f ? -1.f : 0.f, size = p.scale == 0.f ? 1.f : fabsf(p.scale);
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const int r = rt * ROWS + nt * 8 + g;
@@ -502,7 +561,7 @@ __global__ void __launch_bounds__(kWarps * 32) decode_attention_kernel(const __g
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        x[gr][e] *= kc[d + e];
+        x[gr][e] *= kc[d + e] * sign;
         amax = fmaxf(amax, fabsf(x[gr][e]));
       }
     }
@@ -525,9 +584,10 @@ __global__ void __launch_bounds__(kWarps * 32) decode_attention_kernel(const __g
       qb[nt][gr][3] = pack_half2(x[gr][3] * 0.0625f, x[gr][7] * 0.0625f);
       z += __shfl_xor_sync(0xffffffffu, z, 1);
       z += __shfl_xor_sync(0xffffffffu, z, 2);
-      zg[gr] = z * 0.015625f;      // 2^-6: within fp16
+      zg[gr] = z * 5.9604645e-8f;  // 2^-24, the unit of the codes' products
     }
-    // the groups' sums of q' for the zero term, as fp16 high and low parts (22 bits)
+    // the groups' sums of q' for the zero term, as fp16 high and low parts: together exact to
+    // half a unit of q', below q's own rounding
     float z0, z1;
     bool low;
     if constexpr (NG == 4) {
@@ -541,7 +601,7 @@ __global__ void __launch_bounds__(kWarps * 32) decode_attention_kernel(const __g
     }
     const float h0 = __half2float(__float2half_rn(z0)), h1 = __half2float(__float2half_rn(z1));
     zb[nt] = low ? pack_half2(z0 - h0, z1 - h1) : pack_half2(h0, h1);
-    const float f = p.scale * kLog2e * 64.f * __uint_as_float((uint32_t)(eb - 13) << 23);
+    const float f = size * kLog2e * 16777216.f * __uint_as_float((uint32_t)(eb - 13) << 23);
     fr[nt][0] = __shfl_sync(0xffffffffu, f, 8 * t4);        // rows 2 t4 and 2 t4 + 1: the lanes that hold them as g
     fr[nt][1] = __shfl_sync(0xffffffffu, f, 8 * t4 + 4);
   }
@@ -558,14 +618,16 @@ __global__ void __launch_bounds__(kWarps * 32) decode_attention_kernel(const __g
   }
   int fe = 14;                     // the V scales are multiplied by 2^fe so that the largest lies below 2
 
+  // the zero term's A rows: 0 .. NG-1 the groups' zeros, 4 ones, the others nothing
+  const uint32_t zkeep = g < NG ? 0xffffffffu : 0u, zone = g == 4 ? 0x3C003C00u : 0u;
   // ldmatrix rows of this lane: matrix mi = lane / 8 covers slots 8 (mi & 1) .. + 7 of group mi / 2
   const int lm_slot = (lane & 7) + ((lane >> 3) & 1) * 8, lm_grp = lane >> 4;
 
   int stage = 0;                   // ring stage of tile i; tile i + kStages - 1 goes into the one before it
-  for (int i = warp; i < tiles; i += kWarps) {
-    const int nx = i + (kStages - 1) * kWarps;
-    flight[kStages - 1] = issue(nx, stage == 0 ? kStages - 1 : stage - 1, sb, sj);
-    resolve(nx + kWarps, sb, sj);
+  for (int i = warp; i < tiles; i += W) {
+    const int nx = i + (kStages - 1) * W;
+    flight[kStages - 1] = issue(nx, stage == 0 ? kStages - 1 : stage - 1, next);
+    next = find(nx + W);
     cp_wait<kStages - 1>();
     __syncwarp();
     const uint32_t st = ring + stage * R::kStage;
@@ -578,7 +640,6 @@ __global__ void __launch_bounds__(kWarps * 32) decode_attention_kernel(const __g
     float sc[2][NT][4];
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) {
-      constexpr int kSc = D / 16;
       const uint32_t sa = st + (mt * 16 + g) * kSc;
       float s0[NG], s1[NG];
       if constexpr (NG == 4) {
@@ -593,7 +654,7 @@ __global__ void __launch_bounds__(kWarps * 32) decode_attention_kernel(const __g
       const uint32_t za = sa + R::kKz + (NG == 4 ? (t4 & 1) * 4 : 0);
       const uint32_t z0 = lds32(za), z1 = lds32(za + 8 * kSc);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) sc[mt][nt][0] = sc[mt][nt][1] = sc[mt][nt][2] = sc[mt][nt][3] = 0.f;
+      for (int nt = 0; nt < NT; ++nt) mma8(sc[mt][nt], z0, z1, zb[nt]);
 #pragma unroll
       for (int gp = 0; gp < NG / 2; ++gp) {
         uint32_t w[4];
@@ -604,8 +665,8 @@ __global__ void __launch_bounds__(kWarps * 32) decode_attention_kernel(const __g
           const uint32_t wa = w[2 * e], wb = w[2 * e + 1], xa = wa >> 8, xb = wb >> 8;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            float c[4] = {0.f, 0.f, 0.f, 0.f};
-            mma16(c, wa & 0x000F000Fu, wb & 0x000F000Fu, wa & 0x00F000F0u, wb & 0x00F000F0u, qb[nt][gr][0], qb[nt][gr][1]);
+            float c[4];
+            mma16_set(c, wa & 0x000F000Fu, wb & 0x000F000Fu, wa & 0x00F000F0u, wb & 0x00F000F0u, qb[nt][gr][0], qb[nt][gr][1]);
             mma16(c, xa & 0x000F000Fu, xb & 0x000F000Fu, xa & 0x00F000F0u, xb & 0x00F000F0u, qb[nt][gr][2], qb[nt][gr][3]);
             sc[mt][nt][0] = fmaf(s0[gr], c[0], sc[mt][nt][0]);
             sc[mt][nt][1] = fmaf(s0[gr], c[1], sc[mt][nt][1]);
@@ -613,14 +674,6 @@ __global__ void __launch_bounds__(kWarps * 32) decode_attention_kernel(const __g
             sc[mt][nt][3] = fmaf(s1[gr], c[3], sc[mt][nt][3]);
           }
         }
-      }
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float c[4] = {0.f, 0.f, 0.f, 0.f};
-        mma8(c, z0, z1, zb[nt]);
-        // the codes' part is in units of 2^-24, the zeros' in 2^6
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sc[mt][nt][e] = fmaf(sc[mt][nt][e], 262144.f, c[e]) * fr[nt][e & 1];
       }
     }
     if (alive != 0xffffffffu) {
@@ -634,7 +687,6 @@ __global__ void __launch_bounds__(kWarps * 32) decode_attention_kernel(const __g
     }
 
     // ---- the tile's largest V scale, as an exponent
-    constexpr int kSc = D / 16;
     uint32_t top;
     if constexpr (NG == 4) {
       const uint2 u = lds64(st + R::kVs + lane * kSc);
@@ -666,14 +718,16 @@ __global__ void __launch_bounds__(kWarps * 32) decode_attention_kernel(const __g
         v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
         const float mn = fmaxf(m[nt][c], v);
         const float ms = mn == -INFINITY ? 0.f : mn;
-        corr[nt][c] = ex2(m[nt][c] - ms);
+        corr[nt][c] = ex2((m[nt][c] - ms) * fr[nt][c]);
         m[nt][c] = mn;
-        off[c] = 14.f - ms;
+        off[c] = fmaf(-ms, fr[nt][c], 14.f);
       }
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt) {
-        pb[mt][nt][0] = transpose8x8(pack_half2(ex2(sc[mt][nt][0] + off[0]), ex2(sc[mt][nt][1] + off[1])));
-        pb[mt][nt][1] = transpose8x8(pack_half2(ex2(sc[mt][nt][2] + off[0]), ex2(sc[mt][nt][3] + off[1])));
+        pb[mt][nt][0] = transpose8x8(pack_half2(ex2(fmaf(sc[mt][nt][0], fr[nt][0], off[0])),
+                                                 ex2(fmaf(sc[mt][nt][1], fr[nt][1], off[1]))));
+        pb[mt][nt][1] = transpose8x8(pack_half2(ex2(fmaf(sc[mt][nt][2], fr[nt][0], off[0])),
+                                                 ex2(fmaf(sc[mt][nt][3], fr[nt][1], off[1]))));
       }
     }
 
@@ -685,13 +739,12 @@ __global__ void __launch_bounds__(kWarps * 32) decode_attention_kernel(const __g
 #pragma unroll
         for (int hb = 0; hb < 2; ++hb) {
           const uint32_t za = st + R::kVz + (mt * 16 + hb * 8 + 2 * t4) * kSc + (g & (NG - 1)) * 2;
-          const uint32_t v = lds16(za) | lds16(za + kSc) << 16;
-          a[mt][hb] = g < NG ? v : g == 4 ? 0x3C003C00u : 0u;
+          a[mt][hb] = (__byte_perm(lds16(za), lds16(za + kSc), 0x5410) & zkeep) | zone;
         }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float c[4] = {0.f, 0.f, 0.f, 0.f};
-        mma16(c, a[0][0], 0u, a[0][1], 0u, pb[0][nt][0], pb[0][nt][1]);
+        float c[4];
+        mma16_set(c, a[0][0], 0u, a[0][1], 0u, pb[0][nt][0], pb[0][nt][1]);
         mma16(c, a[1][0], 0u, a[1][1], 0u, pb[1][nt][0], pb[1][nt][1]);
         zl[nt][0] = fmaf(zl[nt][0], corr[nt][0], c[0]);
         zl[nt][1] = fmaf(zl[nt][1], corr[nt][1], c[1]);
@@ -731,13 +784,18 @@ __global__ void __launch_bounds__(kWarps * 32) decode_attention_kernel(const __g
         const int gr = gp * 2 + e;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          float c0[4] = {0.f, 0.f, 0.f, 0.f}, c1[4] = {0.f, 0.f, 0.f, 0.f};
+          float c0[4], c1[4];
 #pragma unroll
           for (int mt = 0; mt < 2; ++mt) {
             const uint32_t b0 = hmul2(pb[mt][nt][0], vsc[mt][0][gr]), b1 = hmul2(pb[mt][nt][1], vsc[mt][1][gr]);
             const uint32_t xa = x[mt][2 * e], xb = x[mt][2 * e + 1], ya = xa >> 8, yb = xb >> 8;
-            mma16(c0, xa & 0x000F000Fu, xa & 0x00F000F0u, xb & 0x000F000Fu, xb & 0x00F000F0u, b0, b1);
-            mma16(c1, ya & 0x000F000Fu, ya & 0x00F000F0u, yb & 0x000F000Fu, yb & 0x00F000F0u, b0, b1);
+            if (mt == 0) {
+              mma16_set(c0, xa & 0x000F000Fu, xa & 0x00F000F0u, xb & 0x000F000Fu, xb & 0x00F000F0u, b0, b1);
+              mma16_set(c1, ya & 0x000F000Fu, ya & 0x00F000F0u, yb & 0x000F000Fu, yb & 0x00F000F0u, b0, b1);
+            } else {
+              mma16(c0, xa & 0x000F000Fu, xa & 0x00F000F0u, xb & 0x000F000Fu, xb & 0x00F000F0u, b0, b1);
+              mma16(c1, ya & 0x000F000Fu, ya & 0x00F000F0u, yb & 0x000F000Fu, yb & 0x00F000F0u, b0, b1);
+            }
           }
           const float k0 = corr[nt][0] * down, k1 = corr[nt][1] * down;
           float* oo = o[nt][gr];
@@ -759,8 +817,8 @@ __global__ void __launch_bounds__(kWarps * 32) decode_attention_kernel(const __g
 
   // ---- the warps' rows to shared memory (over the rings): o = codes' part + zeros' part, both
   // from units of 2^14 p
-  float* sRows = reinterpret_cast<float*>(smem);
-  float2* sML = reinterpret_cast<float2*>(smem + kWarps * ROWS * kPad * 4);
+  float2* sML = reinterpret_cast<float2*>(smem);
+  float* sRows = reinterpret_cast<float*>(smem + W * ROWS * 8);
   const float unit = __uint_as_float((uint32_t)(127 + 10 - fe) << 23);       // 2^(24 - 14 - fe)
   constexpr float kZ = 1.f / 16384.f;
 #pragma unroll
@@ -778,36 +836,61 @@ __global__ void __launch_bounds__(kWarps * 32) decode_attention_kernel(const __g
           make_float4(fmaf(oo[1], unit, zc), fmaf(oo[3], unit * 0.0625f, zc), fmaf(oo[5], unit, zc), fmaf(oo[7], unit * 0.0625f, zc));
     }
     if (g == 4) {       // the ones' row of the zero-term products: the row sums
-      sML[warp * ROWS + nt * 8 + 2 * t4] = make_float2(m[nt][0], zl[nt][0] * kZ);
-      sML[warp * ROWS + nt * 8 + 2 * t4 + 1] = make_float2(m[nt][1], zl[nt][1] * kZ);
+      sML[warp * ROWS + nt * 8 + 2 * t4] = make_float2(m[nt][0] * fr[nt][0], zl[nt][0] * kZ);
+      sML[warp * ROWS + nt * 8 + 2 * t4 + 1] = make_float2(m[nt][1] * fr[nt][1], zl[nt][1] * kZ);
     }
   }
   __syncthreads();
-  finish<D, ROWS>(p, s, h, rt, blockIdx.x, kWarps, sRows, sML);
+  finish<D, ROWS, W>(p, s, h, rt, blockIdx.x, W, sRows, sML, sML);
 }
 
-template <int D, int NT>
+template <int D, int NT, int W>
 constexpr size_t decode_smem() {
-  const size_t ring = (size_t)kWarps * Ring<D>::kWarpBytes;
-  const size_t rows = (size_t)kWarps * 8 * NT * ((D + 4) * 4 + 8);
-  const size_t merge = (size_t)8 * NT * (kWarps * 32 / (D / 4)) * (D + 4) * 4;
-  const size_t block = (size_t)8 * NT * (D + 4) * 4 + 2 * 32 * (D + 8) * 2 + 8 * NT * 8;
-  size_t most = ring > rows ? ring : rows;
-  most = most > merge ? most : merge;
+  const size_t ring = (size_t)W * Ring<D>::kWarpBytes;
+  const size_t rows = (size_t)W * 8 * NT * ((D + 4) * 4 + 8);
+  const size_t block = (size_t)W * 8 * NT * 8 + (size_t)8 * NT * (D + 4) * 4 + 2 * 32 * (D + 8) * 2;
+  const size_t most = ring > rows ? ring : rows;
   return most > block ? most : block;
 }
 
-template <int D, int NT>
+template <int D, int NT, int W, int MINB, bool FAST>
 int launch(const DecodeParams& p, cudaStream_t st) {
-  constexpr size_t smem = decode_smem<D, NT>();
-  if (cudaFuncSetAttribute(decode_attention_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-    return MA_ERR_CUDA;
-  const dim3 grid(p.slots, p.H * p.row_tiles);
-  decode_attention_kernel<D, NT><<<grid, kWarps * 32, smem, st>>>(p);
+  constexpr size_t smem = decode_smem<D, NT, W>();
+  auto kernel = decode_attention_kernel<D, NT, W, MINB, FAST>;
+  static bool ready[64] = {false};       // per device: the attributes are set once
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return MA_ERR_CUDA;
+  if (dev < 0 || dev >= 64 || !ready[dev]) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
+        cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) != cudaSuccess)
+      return MA_ERR_CUDA;
+    if (dev >= 0 && dev < 64) ready[dev] = true;
+  }
+  kernel<<<dim3(p.slots, p.H * p.row_tiles), W * 32, smem, st>>>(p);
   return cudaGetLastError() == cudaSuccess ? MA_OK : MA_ERR_CUDA;
 }
 
-int rows_per_tile(int R) { return R <= 8 ? 8 : R <= 16 ? 16 : 32; }
+// Tiles that are contiguous in storage: positions packed back to back, K and V arrays of one
+// geometry, 32-slot tiles that do not straddle pages, scale blocks on 16-byte boundaries.
+bool contiguous_tiles(const ma_kv& kv, int D) {
+  if (kv.mask != nullptr) return false;
+  if (kv.pages != nullptr && kv.page_size % kTile != 0) return false;
+  if (kv.skq[2] != D / 2 || kv.sks[2] != D / 32) return false;
+  for (int i = 0; i < 3; ++i)
+    if (kv.skq[i] != kv.svq[i] || kv.sks[i] != kv.svs[i] || (i < 2 && kv.sks[i] % 8 != 0)) return false;
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(kv.ks) | reinterpret_cast<uintptr_t>(kv.kz) |
+                         reinterpret_cast<uintptr_t>(kv.vs) | reinterpret_cast<uintptr_t>(kv.vz);
+  return (bits & 15) == 0;
+}
+
+int rows_per_tile(int R) { return R <= 8 ? 8 : 16; }
+
+template <int D>
+int launch_rows(const DecodeParams& p, cudaStream_t st) {
+  const bool fast = contiguous_tiles(p.kv, D);
+  if (rows_per_tile(p.R) == 8) return fast ? launch<D, 1, 8, 2, true>(p, st) : launch<D, 1, 8, 2, false>(p, st);
+  return fast ? launch<D, 2, 8, 1, true>(p, st) : launch<D, 2, 8, 1, false>(p, st);
+}
 
 }  // namespace
 
@@ -824,15 +907,9 @@ void plan_decode(int B, int H, int R, int Tc, DecodePlan& plan) {
 }
 
 int launch_decode_attention(DecodeParams& p, cudaStream_t st) {
-  const int nt = rows_per_tile(p.R) / 8;
-  if (p.D == 128) {
-    if (nt == 1) return launch<128, 1>(p, st);
-    if (nt == 2) return launch<128, 2>(p, st);
-    return launch<128, 4>(p, st);
-  }
-  if (nt == 1) return launch<64, 1>(p, st);
-  if (nt == 2) return launch<64, 2>(p, st);
-  return launch<64, 4>(p, st);
+  p.tiles_per_page = p.kv.pages != nullptr ? p.kv.page_size / kTile : 1;
+  p.tile_div.set(p.tiles_per_page > 0 ? p.tiles_per_page : 1);
+  return p.D == 128 ? launch_rows<128>(p, st) : launch_rows<64>(p, st);
 }
 
 }  // namespace ma

@@ -189,6 +189,18 @@ int launch_head_gather(const void* part, const int64_t sp[3], int B, int Hl, int
 // device properties, cached per device
 int device_sm_count();
 
+// n / d for 0 <= n < 2^31 and a divisor known to the host: q = (umulhi(n, mul) + n) >> shift
+// (Granlund and Montgomery's multiplication by an invariant)
+struct FastDiv {
+  uint32_t mul, shift;
+  void set(uint32_t d) {
+    shift = 0;
+    while (shift < 31 && (1u << shift) < d) ++shift;
+    mul = (uint32_t)(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
+  }
+  __device__ __forceinline__ int div(int n) const { return (int)((__umulhi((uint32_t)n, mul) + (uint32_t)n) >> shift); }
+};
+
 // ma_decode.cu: attention of few bf16 rows over a token-mode k4v4 cache read in place
 struct DecodeParams {
   const __nv_bfloat16* q;
@@ -205,8 +217,10 @@ struct DecodeParams {
   float* acc;          // [H][row tiles][slots][rows][D] their unnormalized outputs
   int slots;           // splits per (head, row tile): the grid's x extent
   int target;          // chunks the live slots are spread over
-  int min_units;       // shortest chunk, in 128-slot units
+  int min_units;       // shortest chunk, in units of its granularity
   int row_tiles;
+  int tiles_per_page;  // 32-slot tiles
+  FastDiv tile_div;    // by tiles_per_page
 };
 struct DecodePlan {
   int rows, row_tiles, target, slots;

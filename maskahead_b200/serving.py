@@ -21,11 +21,12 @@ tensor of decode_workspace_bytes / verify_workspace_bytes / PLAN_WORKSPACE_BYTES
 
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _lib
 from ._lib import MaBlock, MaRows, i64
-from .kernels._common import block_struct, rows_struct
 from .layouts import Prefix, as_prefix, kv_descriptor
 
 __all__ = ["PagedCache", "TokenPlan", "decode_attention", "verify_drafts", "decode_workspace_bytes",
@@ -53,12 +54,13 @@ def decode_workspace_bytes(batch: int, heads: int, rows: int, head_dim: int, blo
     return int(_lib.load_library().ma_decode_attention_workspace(batch, heads, rows, head_dim, block_tokens))
 
 
+@functools.lru_cache(maxsize=256)
 def verify_workspace_bytes(batch: int, vocab: int) -> int:
     return int(_lib.load_library().ma_verify_drafts_workspace(batch, vocab))
 
 
 def _check(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple, device: torch.device) -> None:
-    if t.dtype != dtype or tuple(t.shape) != shape or t.device != device or not t.is_contiguous():
+    if t.dtype != dtype or t.shape != shape or t.device != device or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape} on {device}, "
                          f"got {t.dtype} {tuple(t.shape)} on {t.device}")
 
@@ -158,7 +160,7 @@ class PagedCache:
                 raise ValueError("a cache's tensors must lie on one device")
         self._desc = kv_descriptor(self.prefix())       # checks types and strides
         self._lib = _lib.lib()
-        self._bytes: dict[tuple, int] = {}
+        self._forms: dict[tuple, _Call] = {}            # attention calls' forms that passed their checks
 
     @classmethod
     def allocate(cls, *, batch: int, heads: int, head_dim: int, num_pages: int, page_size: int, max_pages: int,
@@ -196,23 +198,22 @@ class PagedCache:
         [N, H, D] in the rows' type."""
         if key.ndim != 3 or key.shape != value.shape or key.dtype != value.dtype:
             raise ValueError("key and value must be [N, H, D] tensors of one shape and type")
-        n = key.shape[0]
-        if tuple(key.shape[1:]) != (self.heads, self.head_dim):
+        n, heads, dim = key.shape
+        dev = self.device
+        if heads != self.heads or dim != self.head_dim:
             raise ValueError(f"rows must be [N, {self.heads}, {self.head_dim}]")
-        if key.device != self.device or value.device != self.device:
-            raise ValueError(f"rows must lie on {self.device}")
-        _check("slots", slots, torch.int64, (n,), self.device)
-        _check("seqs", seqs, torch.int32, (n,), self.device)
-        code = _lib.dtype_code(key.dtype)
-        k, v = _rows3(key), _rows3(value)
+        if key.device != dev or value.device != dev:
+            raise ValueError(f"rows must lie on {dev}")
+        _check("slots", slots, torch.int64, (n,), dev)
+        _check("seqs", seqs, torch.int32, (n,), dev)
+        k, v = _aligned(key), _aligned(value)
         rows_k = rows_v = None
         if return_rows:
-            rows_k = torch.empty((n, self.heads, self.head_dim), device=self.device, dtype=key.dtype)
-            rows_v = torch.empty_like(rows_k)
+            rows_k, rows_v = torch.empty((2, n, heads, dim), device=dev, dtype=key.dtype).unbind(0)
         rc = self._lib.ma_append_tokens(
-            self._desc.kv, self.batch, self.heads, self.head_dim, k.data_ptr(), v.data_ptr(), code, n,
-            i64(*k.stride()[:2]), i64(*v.stride()[:2]), slots.data_ptr(), seqs.data_ptr(), _lib.ptr(rows_k),
-            _lib.ptr(rows_v), _lib.stream_handle(self.device))
+            self._desc.kv, self.batch, heads, dim, k.data_ptr(), v.data_ptr(), _lib.dtype_code(key.dtype), n,
+            _strides(k.stride()[:2]), _strides(v.stride()[:2]), slots.data_ptr(), seqs.data_ptr(), _lib.ptr(rows_k),
+            _lib.ptr(rows_v), _lib.stream_handle(dev))
         if rc:
             _lib.check("ma_append_tokens", rc)
         return (rows_k, rows_v) if return_rows else None
@@ -224,11 +225,18 @@ class PagedCache:
         return _attend(query, self, self._desc, current_key, current_value, scaling, causal, out, workspace)
 
 
-def _rows3(t: torch.Tensor) -> torch.Tensor:
-    """[N, H, D] rows with a contiguous, 16-byte aligned last axis, copying if not."""
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """t with a contiguous last axis and every row on a 16-byte boundary, copied if it is not."""
     es = t.element_size()
-    ok = t.stride(2) == 1 and t.data_ptr() % 16 == 0 and (t.stride(0) * es) % 16 == 0 and (t.stride(1) * es) % 16 == 0
-    return t if ok else t.contiguous()
+    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s * es % 16 == 0 for s in t.stride()[:-1]):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+@functools.lru_cache(maxsize=1024)
+def _strides(pair: tuple):
+    """Two strides as the C ABI takes them (never written to, so calls may share them)."""
+    return i64(*pair)
 
 
 # ----------------------------------------------------------------------------- attention
@@ -251,21 +259,87 @@ def decode_attention(query: torch.Tensor, prefix, current_key: torch.Tensor | No
     return _attend(query, pre, None, current_key, current_value, scaling, causal, out, workspace)
 
 
+class _Call:
+    """What one form of an in-place attention call (its tensors' shapes, strides and types)
+    passes besides the pointers."""
+
+    __slots__ = ("heads", "geometry", "sq", "tc", "sk", "sv", "shape", "so", "scale", "causal", "nbytes")
+
+
+_MAX_FORMS = 256     # remembered forms per cache; a loop has a few
+
+
 def _attend(query, source, desc, current_key, current_value, scaling, causal, out, workspace):
+    """decode_attention. The checks below depend on shapes, strides, types and devices alone, so
+    a PagedCache remembers the forms that passed them (the checks and descriptors took 28 us
+    of host time a call, the kernel of a single token over 8192 slots a third of that)."""
+    forms = form = call = None
+    if isinstance(source, PagedCache):
+        forms = source._forms
+        form = (query.shape, query.stride(), query.dtype, query.device, scaling, causal,
+                None if current_key is None else (current_key.shape, current_key.stride(), current_key.dtype,
+                                                  current_key.device),
+                None if current_value is None else (current_value.shape, current_value.stride(), current_value.dtype,
+                                                    current_value.device),
+                None if out is None else (out.shape, out.stride(), out.dtype, out.device))
+        call = forms.get(form)
+    if call is None:
+        if query.dtype == torch.bfloat16 and current_value is not None and current_key is not None:
+            k2, v2 = _aligned(current_key.to(query.dtype)), _aligned(current_value.to(query.dtype))
+        else:
+            k2, v2 = current_key, current_value
+        q2 = _aligned(query)
+        if q2 is not query or k2 is not current_key or v2 is not current_value:
+            return _attend(q2, source, desc, k2, v2, scaling, causal, out, workspace)
+        call = _attend_form(query, source, current_key, current_value, scaling, causal, out)
+        if call is None:
+            return _attend_general(query, source, current_key, current_value, scaling, causal, out)
+        if forms is not None:
+            if len(forms) >= _MAX_FORMS:
+                forms.clear()
+            forms[form] = call
+    q = query.data_ptr()
+    k = v = 0
+    if call.tc:
+        k, v = current_key.data_ptr(), current_value.data_ptr()
+    if (q | k | v) & 15:       # strides that can be read, but a start between 16-byte boundaries
+        if k | v:
+            current_key, current_value = _aligned(current_key), _aligned(current_value)
+        return _attend(_aligned(query), source, desc, current_key, current_value, scaling, causal, out, workspace)
+    if out is not None and out.data_ptr() & 15:
+        raise ValueError("out must start on a 16-byte boundary")
+    if desc is None:
+        desc = kv_descriptor(source, batch=query.shape[0], heads=call.heads, head_dim=query.shape[3])
+    o = torch.empty(call.shape, device=query.device, dtype=query.dtype) if out is None else out
+    ws = _workspace(query.device, "decode", call.nbytes, workspace)
+    rc = _lib.lib().ma_decode_attention(
+        MaRows(q, _lib.MA_BF16, *call.geometry, call.sq), desc.kv, call.heads, MaBlock(k, v, call.tc, call.sk, call.sv),
+        call.scale, call.causal, o.data_ptr(), call.so, ws.data_ptr(), ws.numel(), _lib.stream_handle(query.device))
+    if rc == _lib.MA_ERR_UNSUPPORTED:
+        return _attend_general(query, source, current_key, current_value, scaling, causal, out)
+    if rc:
+        _lib.check("ma_decode_attention", rc)
+    return o
+
+
+def _attend_form(query, source, current_key, current_value, scaling, causal, out) -> _Call | None:
+    """Check a call; its _Call when it is read in place, None for the general route."""
     if query.ndim != 4:
         raise ValueError("query must have shape [B, Hq, T, D]")
+    if not query.is_cuda:
+        raise _lib.KernelUnavailableError("maskahead_b200 kernels need CUDA tensors")
     b, hq, t, d = query.shape
     tc = 0 if current_key is None else current_key.shape[2]
-    if current_key is not None and (current_value is None or current_key.shape != current_value.shape
-                                    or current_key.ndim != 4):
+    if (current_key is None) != (current_value is None) or current_key is not None and (
+            current_key.shape != current_value.shape or current_key.ndim != 4):
         raise ValueError("current K and V must be [B, Hkv, Tc, D] tensors of one shape")
     if causal and 0 < tc < t:
         raise ValueError(f"causal rows need at least as many current keys as rows: Tc={tc} < T={t}")
     cached = isinstance(source, PagedCache)
     if cached:
         heads = source.heads
-        if b != source.batch or d != source.head_dim:
-            raise ValueError(f"query must be [{source.batch}, Hq, T, {source.head_dim}]")
+        if b != source.batch or d != source.head_dim or query.device != source.device:
+            raise ValueError(f"query must be [{source.batch}, Hq, T, {source.head_dim}] on {source.device}")
     else:
         stored = source.kf if source.kf is not None else source.vq
         if stored is None and current_key is None:
@@ -273,45 +347,26 @@ def _attend(query, source, desc, current_key, current_value, scaling, causal, ou
         heads = current_key.shape[1] if stored is None else stored.shape[1]
     if hq % heads:
         raise ValueError("Hq must be divisible by Hkv")
-    if current_key is not None and (current_key.shape[0] != b or current_key.shape[1] != heads
-                                    or current_key.shape[3] != d):
-        raise ValueError(f"current K and V must be [{b}, {heads}, Tc, {d}]")
-    rows = hq // heads * t
+    if current_key is not None and (tuple(current_key.shape) != (b, heads, tc, d) or current_key.device != query.device
+                                    or current_value.device != query.device):
+        raise ValueError(f"current K and V must be [{b}, {heads}, Tc, {d}] on {query.device}")
     if out is not None and (out.shape != query.shape or out.dtype != query.dtype or out.device != query.device
-                            or out.stride(-1) != 1):
-        raise ValueError("out must match the query's shape, type and device, with a contiguous head_dim")
-    lib = _lib.lib()
-    if query.dtype == torch.bfloat16 and rows <= MAX_DECODE_ROWS and (
+                            or out.stride(-1) != 1 or any(s * out.element_size() % 16 for s in out.stride()[:3])):
+        raise ValueError("out must match the query's shape, type and device, with contiguous rows on 16-byte boundaries")
+    rows = hq // heads * t
+    if query.dtype != torch.bfloat16 or rows > MAX_DECODE_ROWS or not (
             cached or (source.nq > 0 and source.nf == 0 and source.kmode == 1)):
-        if desc is None:
-            desc = kv_descriptor(source, batch=b, heads=heads, head_dim=d)
-        r, q = _rows(query)
-        blk, keep = _block(current_key, current_value)
-        o = torch.empty((b, hq, t, d), device=query.device, dtype=query.dtype) if out is None else out
-        key = (b, heads, rows, d, tc)
-        nbytes = source._bytes.get(key) if cached else None
-        if nbytes is None:
-            nbytes = lib.ma_decode_attention_workspace(*key)
-            if cached:
-                source._bytes[key] = nbytes
-        ws = _workspace(query.device, "decode", nbytes, workspace)
-        rc = lib.ma_decode_attention(r, desc.kv, heads, blk, d ** -0.5 if scaling is None else float(scaling),
-                                     1 if causal else 0, o.data_ptr(), i64(*o.stride()[:3]), ws.data_ptr(), ws.numel(),
-                                     _lib.stream_handle(query.device))
-        if rc == _lib.MA_OK:
-            return o
-        if rc != _lib.MA_ERR_UNSUPPORTED:
-            _lib.check("ma_decode_attention", rc)
-        del q, keep
-    return _attend_general(query, source, current_key, current_value, scaling, causal, out)
-
-
-def _rows(query: torch.Tensor):
-    return rows_struct(query)
-
-
-def _block(key, value):
-    return block_struct(key, value, torch.bfloat16)
+        return None
+    call = _Call()
+    call.heads, call.geometry, call.tc = heads, (b, hq, t, d), tc
+    call.sq = i64(*query.stride()[:3])
+    call.sk, call.sv = (i64(*current_key.stride()[:3]), i64(*current_value.stride()[:3])) if tc else (i64(0, 0, 0), i64(0, 0, 0))
+    call.shape = (b, hq, t, d)
+    call.so = i64(hq * t * d, t * d, d) if out is None else i64(*out.stride()[:3])
+    call.scale = d ** -0.5 if scaling is None else float(scaling)
+    call.causal = 1 if causal else 0
+    call.nbytes = int(_lib.lib().ma_decode_attention_workspace(b, heads, rows, d, tc))
+    return call
 
 
 def _attend_general(query, source, current_key, current_value, scaling, causal, out):
@@ -358,7 +413,7 @@ def verify_drafts(target: torch.Tensor, draft: torch.Tensor | None, tokens: torc
         raise ValueError("target must be [B, K + 1, V] with B, V >= 1 and K >= 0")
     if target.stride(2) != 1 and v > 1:
         raise ValueError("target must have a contiguous vocabulary axis")
-    if draft is not None and (draft.dtype != target.dtype or tuple(draft.shape) != (b, k, v) or draft.device != dev
+    if draft is not None and (draft.dtype != target.dtype or draft.shape != (b, k, v) or draft.device != dev
                               or (draft.stride(2) != 1 and v > 1)):
         raise ValueError(f"draft must be a {target.dtype} tensor {(b, k, v)} on {dev} with a contiguous vocabulary axis")
     _check("tokens", tokens, torch.int32, (b, k), dev)
@@ -368,10 +423,10 @@ def verify_drafts(target: torch.Tensor, draft: torch.Tensor | None, tokens: torc
     lib = _lib.lib()
     accepted = torch.empty(b, device=dev, dtype=torch.int32)
     out = torch.empty((b, k1), device=dev, dtype=torch.int32)
-    ws = _workspace(dev, "verify", lib.ma_verify_drafts_workspace(b, v), workspace)
+    ws = _workspace(dev, "verify", verify_workspace_bytes(b, v), workspace)
     code = _lib.MA_F16 if target.dtype == torch.float16 else _lib.dtype_code(target.dtype)
-    rc = lib.ma_verify_drafts(target.data_ptr(), _lib.ptr(draft), code, b, k, v, i64(target.stride(0), target.stride(1)),
-                              i64(draft.stride(0), draft.stride(1)) if draft is not None else None,
+    rc = lib.ma_verify_drafts(target.data_ptr(), _lib.ptr(draft), code, b, k, v, _strides(target.stride()[:2]),
+                              _strides(draft.stride()[:2]) if draft is not None else None,
                               tokens.data_ptr(), _lib.ptr(counts), uniforms.data_ptr(), accepted.data_ptr(),
                               out.data_ptr(), ws.data_ptr(), ws.numel(), _lib.stream_handle(dev))
     if rc:
