@@ -769,12 +769,6 @@ inline char* align256(void* ws) {
   return reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(ws) + 255) & ~uintptr_t(255));
 }
 
-size_t decode_scratch(int H, int D, const DecodePlan& d, size_t& ml) {
-  const size_t splits = (size_t)H * d.row_tiles * d.slots * d.rows;
-  ml = (splits * sizeof(float2) + 255) & ~(size_t)255;
-  return ml + splits * D * sizeof(float);
-}
-
 // a pool (or contiguous cache) of token-mode k4v4 rows without a dense tail whose scale and
 // zero rows a copy of their own size can read
 bool packed_in_place(const ma_kv& kv, int D) {
@@ -793,10 +787,8 @@ bool packed_in_place(const ma_kv& kv, int D) {
 
 size_t ma_decode_attention_workspace(int B, int H, int R, int D, int Tc) {
   if (B <= 0 || H <= 0 || R <= 0 || D <= 0 || Tc < 0) return 0;
-  DecodePlan d;
-  plan_decode(B, H, R, Tc, d);
   size_t ml;
-  return 512 + kDecodeTickets * sizeof(unsigned) + decode_scratch(H, D, d, ml);
+  return 512 + kDecodeTickets * sizeof(unsigned) + decode_partials(H, R, D, ml);
 }
 
 int ma_decode_attention(const ma_rows* q, const ma_kv* kv, int H, const ma_block* cur, float scale, int causal,
@@ -814,11 +806,11 @@ int ma_decode_attention(const ma_rows* q, const ma_kv* kv, int H, const ma_block
   if ((int64_t)p.G * q->T > 0x7fffffffLL / 64) return MA_ERR_UNSUPPORTED;
   p.R = p.G * q->T;
   DecodePlan d;
-  plan_decode(q->B, H, p.R, cur->Tc, d);
+  plan_decode(q->B, H, p.R, q->D, kv, d);
   if ((int64_t)H * d.row_tiles > 65535 || (int64_t)q->B * H * d.row_tiles > (int64_t)kDecodeTickets)
     return MA_ERR_UNSUPPORTED;
   size_t ml;
-  const size_t scratch = decode_scratch(H, q->D, d, ml);
+  const size_t scratch = decode_partials(H, p.R, q->D, ml);
   if (!workspace || workspace_bytes < 512 + kDecodeTickets * sizeof(unsigned) + scratch) return MA_ERR_WORKSPACE;
   char* base = align256(workspace) + 256;
   p.q = reinterpret_cast<const __nv_bfloat16*>(q->q);
@@ -839,11 +831,7 @@ int ma_decode_attention(const ma_rows* q, const ma_kv* kv, int H, const ma_block
   base += kDecodeTickets * sizeof(unsigned);
   p.ml = reinterpret_cast<float2*>(base);
   p.acc = reinterpret_cast<float*>(base + ml);
-  p.slots = d.slots;
-  p.target = d.target;
-  p.min_units = 1;
-  p.row_tiles = d.row_tiles;
-  return launch_decode_attention(p, (cudaStream_t)stream);
+  return launch_decode_attention(p, d, (cudaStream_t)stream);
 }
 
 size_t ma_page_plan_workspace(void) { return 512; }

@@ -213,20 +213,22 @@ struct DecodeParams {
   __nv_bfloat16* out;
   int64_t so[3];
   unsigned* tickets;   // [B][H][row tiles], zero between calls
-  float2* ml;          // [H][row tiles][slots][rows] (m in log2 units, l) of every split
-  float* acc;          // [H][row tiles][slots][rows][D] their unnormalized outputs
-  int slots;           // splits per (head, row tile): the grid's x extent
-  int target;          // chunks the live slots are spread over
-  int min_units;       // shortest chunk, in units of its granularity
+  float2* ml;          // [H][row tiles][2 ctas][rows] (m in log2 units, l) of every split
+  float* acc;          // [H][row tiles][2 ctas][rows][D] their unnormalized outputs
+  int ctas;            // CTAs per (head, row tile): the grid's x extent
   int row_tiles;
   int tiles_per_page;  // 32-slot tiles
+  int kchan_vec;       // the divisors' rows are 16-byte aligned
   FastDiv tile_div;    // by tiles_per_page
 };
+constexpr int kDecodeTile = 32, kDecodeUnit = 256;   // slots
 struct DecodePlan {
-  int rows, row_tiles, target, slots;
+  int rows, row_tiles, ctas;
+  bool wide, fast;
 };
-void plan_decode(int B, int H, int R, int Tc, DecodePlan& plan);
-int launch_decode_attention(DecodeParams& p, cudaStream_t st);
+void plan_decode(int B, int H, int R, int D, const ma_kv* kv, DecodePlan& plan);
+size_t decode_partials(int H, int R, int D, size_t& ml);
+int launch_decode_attention(DecodeParams& p, const DecodePlan& plan, cudaStream_t st);
 
 // ma_pages.cu: page tables and slot maps from request lengths
 struct PagePlanParams {

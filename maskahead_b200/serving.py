@@ -36,6 +36,8 @@ PLAN_WORKSPACE_BYTES = 512
 
 # Rows per KV head (query heads of the group x tokens) up to which attention reads the packed
 # cache in place; beyond, a prefix is unpacked once and the 128-row tensor-core tiles run.
+# 32 requests x 8192 slots, 4 KV heads, in place against unpacked: 7 rows 45 / 330 us, 35 rows
+# 135 / 562, 63 rows 184 / 564, 112 rows 374 / 331; one request: 12 / 29, 17 / 35, 30 / 36, 37 / 29.
 MAX_DECODE_ROWS = 64
 
 _GROUP = 32
