@@ -1,136 +1,272 @@
 // New tokens' K/V rows quantized into the slots of a packed (token-mode k4v4) pool: keys and
 // values in one launch, through a slot map.
 //
-// Each row's 32-channel groups are quantized exactly as ma_quantize_tokens does it (the same
-// operations rounded to the rows' type in the same order), so a cache filled by prompts in one
-// call and by single tokens in many holds the same bytes. A thread has 8 channels: a group's
-// minimum and maximum meet in two shuffles, its 16 payload bytes are four neighbouring words,
-// and a row of 128 channels is read and written by 16 neighbouring threads.
+// Each row's 32-channel groups are quantized to the bytes that ma_quantize_tokens gives, so a
+// cache filled by prompts in one call and by single tokens in many holds the same. A thread has
+// 8 channels: a group's minimum and maximum meet in two shuffles, its 16 payload bytes are
+// four neighbouring words, and a row of 128 channels is read and written by 16 neighbouring
+// threads. A block takes a run of consecutive tokens, so that a thread keeps its head, its
+// channels and, until the request changes, its divisors and their reciprocals.
 //
-// Bound: HBM (bf16 D = 128: 256 B in, 80 B to the pool, 256 B of values out per row), the launch
-// for a few tokens.
+// Bound: HBM (bf16 D = 128: 256 B in, 80 B to the pool, 256 B of values out per row) with the
+// issue slots close behind: at the copy's rate an SM has about 26 instructions per element and
+// lane. So the bf16 form does without divisions. With 8-bit significands a quotient a / s can
+// neither lie on nor within 2^-17 of a boundary of bf16 rounding (m s = a has no solution for a
+// 9-bit odd m), so a product with a reciprocal that is off by a few ulps rounds to the same
+// bf16. A key's divisor has 24 bits: there the product is checked against the boundary, and the
+// few elements within 4 ulps of it (one in 8000) are divided.
+#include <type_traits>
+
 #include "ma_kernels.cuh"
 
 namespace ma {
 
 namespace {
 
-constexpr int kGroup = 32;
 constexpr int kThreads = 256;
+constexpr int kGroup = 32;
 
-template <bool BF16>
-__device__ __forceinline__ float rnd(float x) {
-  return BF16 ? __bfloat162float(__float2bfloat16_rn(x)) : x;
+// ---- one group's 8 channels of a thread: x (keys already divided) -> codes, step and minimum
+struct Quantized {
+  uint32_t packed;
+  __half step, low;
+  float code[8];
+};
+
+// 32-bit rows: the quantizer's operations as they are.
+__device__ __forceinline__ Quantized quantize(const float x[8]) {
+  float mn = x[0], mx = x[0];
+#pragma unroll
+  for (int e = 1; e < 8; ++e) {
+    mn = fminf(mn, x[e]);
+    mx = fmaxf(mx, x[e]);
+  }
+#pragma unroll
+  for (int o = 1; o < kGroup / 8; o <<= 1) {
+    mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  }
+  const float s = fmaxf((mx - mn) / 15.0f, 1e-8f);
+  Quantized r;
+  r.packed = 0u;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    r.code[e] = fminf(fmaxf(rintf((x[e] - mn) / s), 0.f), 15.f);
+    r.packed |= (uint32_t)r.code[e] << (4 * e);
+  }
+  r.step = __float2half_rn(s);
+  r.low = __float2half_rn(mn);
+  return r;
 }
 
-__device__ __forceinline__ void store8(float* p, const float f[8]) {
+__device__ __forceinline__ uint32_t bits(__nv_bfloat162 x) { return *reinterpret_cast<uint32_t*>(&x); }
+__device__ __forceinline__ __nv_bfloat162 pair(uint32_t x) { return *reinterpret_cast<__nv_bfloat162*>(&x); }
+__device__ __forceinline__ float lo_float(uint32_t x) { return __uint_as_float(x << 16); }
+__device__ __forceinline__ float hi_float(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
+
+// bf16 rows, x in pairs: every operation rounded to bf16, as the quantizer does it.
+__device__ __forceinline__ Quantized quantize(const uint32_t x[4]) {
+  __nv_bfloat162 mn = __hmin2(__hmin2(pair(x[0]), pair(x[1])), __hmin2(pair(x[2]), pair(x[3])));
+  __nv_bfloat162 mx = __hmax2(__hmax2(pair(x[0]), pair(x[1])), __hmax2(pair(x[2]), pair(x[3])));
+#pragma unroll
+  for (int o = 1; o < kGroup / 8; o <<= 1) {
+    mn = __hmin2(mn, pair(__shfl_xor_sync(0xffffffffu, bits(mn), o)));
+    mx = __hmax2(mx, pair(__shfl_xor_sync(0xffffffffu, bits(mx), o)));
+  }
+  const float low = fminf(lo_float(bits(mn)), hi_float(bits(mn))), high = fmaxf(lo_float(bits(mx)), hi_float(bits(mx)));
+  const float d = bf16_round(high - low);
+  // d / 15 rounds to bf16 as d times the rounded 1/15 does (above)
+  const float s = bf16_round(fmaxf(bf16_round(d * (1.0f / 15.0f)), 1e-8f));
+  const float rs = __fdividef(1.0f, s);
+  const __nv_bfloat162 low2 = __float2bfloat162_rn(low);
+  Quantized r;
+  uint32_t c[4];
+  // non-finite rows and steps (s or its reciprocal out of range): the operations as they are
+  const bool plain = d < 1e30f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t a = bits(__hsub2(pair(x[e]), low2));
+    float t0, t1;
+    if (plain) {
+      t0 = lo_float(a) * rs;
+      t1 = hi_float(a) * rs;
+    } else {
+      t0 = lo_float(a) / s;
+      t1 = hi_float(a) / s;
+    }
+    // in [0, 15.1] or NaN (-> 0); 128 + t rounds t to the nearest whole number, ties to even
+    const __nv_bfloat162 t = __hmin2(__hmax2(__floats2bfloat162_rn(t0, t1), __float2bfloat162_rn(0.f)), __float2bfloat162_rn(15.f));
+    c[e] = bits(__hadd2(t, __float2bfloat162_rn(128.f)));
+    r.code[2 * e] = lo_float(c[e]) - 128.f;
+    r.code[2 * e + 1] = hi_float(c[e]) - 128.f;
+    c[e] = (c[e] & 0xfu) | ((c[e] >> 12) & 0xf0u);
+  }
+  r.packed = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+  r.step = __float2half_rn(s);
+  r.low = __float2half_rn(low);
+  return r;
+}
+
+// A thread's divisors: kc, their reciprocals, and whether the products may be used.
+struct Divisors {
+  float kc[8], r[8];
+  bool usable;
+  __device__ __forceinline__ void load(const float* p) {
+    usable = true;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      kc[e] = p[e];
+      r[e] = 1.0f / kc[e];
+      usable &= kc[e] > 1e-30f && kc[e] < 1e30f;
+    }
+  }
+};
+
+__device__ __forceinline__ void divide(const Divisors& k, float x[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] /= k.kc[e];
+}
+__device__ __forceinline__ void divide(const Divisors& k, uint32_t x[4]) {
+  uint32_t near = k.usable ? 0u : 1u;
+  float y[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    y[e] = ((e & 1) ? hi_float(x[e >> 1]) : lo_float(x[e >> 1])) * k.r[e];
+    // within 4 ulps of a boundary of bf16 rounding (0x8000 in the low half)
+    near |= ((__float_as_uint(y[e]) - 0x7ffcu) & 0xffffu) <= 8u ? 1u : 0u;
+  }
+  if (near) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = ((e & 1) ? hi_float(x[e >> 1]) : lo_float(x[e >> 1])) / k.kc[e];
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] = bits(__floats2bfloat162_rn(y[2 * e], y[2 * e + 1]));
+}
+
+__device__ __forceinline__ void load_row(const float* p, float x[8]) { load8(p, x); }
+__device__ __forceinline__ void load_row(const __nv_bfloat16* p, uint32_t x[4]) {
+  const uint4 u = *reinterpret_cast<const uint4*>(p);
+  x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
+}
+__device__ __forceinline__ void store_row(float* p, const float f[8]) {
   reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
   reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
 }
-__device__ __forceinline__ void store8(__nv_bfloat16* p, const float f[8]) {
+__device__ __forceinline__ void store_row(__nv_bfloat16* p, const float f[8]) {
   *reinterpret_cast<uint4*>(p) = float8_to_bf16x8(f);
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant__ AppendParams p, int64_t rows) {
-  constexpr bool BF16 = sizeof(T) == 2;
-  constexpr int kLanes = D / 8;                    // threads per row
-  const int c = threadIdx.x % kLanes, d = c * 8;
-  // rows in the order (token, K or V, head); a warp's rows are a whole number, and every lane
-  // stays in the loop for the shuffles
-  const int64_t step = (int64_t)gridDim.x * kThreads / kLanes;
-  for (int64_t row0 = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / kLanes; __any_sync(0xffffffffu, row0 < rows);
-       row0 += step) {
-    const bool valid = row0 < rows;
-    const int64_t row = valid ? row0 : 0;
-    const int h = (int)(row % p.H);
-    const int64_t rest = row / p.H;
-    const bool key = (rest & 1) == 0;
-    const int64_t i = rest >> 1;
-    const int seq = p.seqs[i];
-    const int64_t slot = p.slots[i];
-    const bool owned = seq >= 0 && seq < p.B;
-    const T* src = reinterpret_cast<const T*>(key ? p.k : p.v);
-    const int64_t* ss = key ? p.sk : p.sv;
-    float x[8], kc[8];
-    load8(src + i * ss[0] + (int64_t)h * ss[1] + d, x);
-    if (key) {
-      const float* q = p.kv.kchan + (int64_t)(owned ? seq : 0) * p.kv.skc[0] + (int64_t)h * p.kv.skc[1] + d;
+template <typename T, int D, bool KEY>
+__device__ __forceinline__ void append_run(const AppendParams& p, int first, int last, int step, int h, int c) {
+  using Raw = typename std::conditional<sizeof(T) == 2, uint32_t, float>::type;
+  constexpr int kRaw = sizeof(T) == 2 ? 4 : 8;
+  const T* src = reinterpret_cast<const T*>(KEY ? p.k : p.v) + (int64_t)h * (KEY ? p.sk[1] : p.sv[1]) + c * 8;
+  const int64_t stride = KEY ? p.sk[0] : p.sv[0];
+  T* rows = reinterpret_cast<T*>(KEY ? p.k_rows : p.v_rows);
+  const int64_t* sq = KEY ? p.kv.skq : p.kv.svq;
+  const int64_t* sc = KEY ? p.kv.sks : p.kv.svs;
+  uint8_t* pay = const_cast<uint8_t*>(KEY ? p.kv.kq : p.kv.vq) + (int64_t)h * sq[1] + c * 4;
+  const int64_t sc0 = (int64_t)h * sc[1] + c / 4;
+  __half* scale = reinterpret_cast<__half*>(const_cast<uint16_t*>(KEY ? p.kv.ks : p.kv.vs)) + sc0;
+  __half* zero = reinterpret_cast<__half*>(const_cast<uint16_t*>(KEY ? p.kv.kz : p.kv.vz)) + sc0;
+  const int64_t limit = (int64_t)p.kv.num_pages * p.kv.page_size;
+
+  Divisors kd;
+  int held = -2;          // the request whose divisors are in kd
+  Raw next[kRaw] = {};
+  int64_t next_slot = -1;
+  int next_seq = -1;
+  auto fetch = [&](int i) {
+    if (i < last) {
+      load_row(src + i * stride, next);
+      next_slot = p.slots[i];
+      next_seq = p.seqs[i];
+    }
+  };
+  fetch(first);
+  // the lanes of a row share its token, and every lane of a warp makes the same number of rounds
+  const int rounds = __reduce_max_sync(0xffffffffu, (unsigned)(last > first ? (last - first + step - 1) / step : 0));
+  for (int k = 0, i = first; k < rounds; ++k, i += step) {
+    Raw x[kRaw];
+#pragma unroll
+    for (int e = 0; e < kRaw; ++e) x[e] = next[e];
+    const int64_t slot = next_slot;
+    const int seq = next_seq;
+    const bool valid = i < last, owned = valid && seq >= 0 && seq < p.B;
+    fetch(i + step);
+    if (KEY) {
+      const int want = owned ? seq : 0;
+      if (want != held) {
+        kd.load(p.kv.kchan + (int64_t)want * p.kv.skc[0] + (int64_t)h * p.kv.skc[1] + c * 8);
+        held = want;
+      }
+      divide(kd, x);
+    }
+    const Quantized q = quantize(x);
+    if (!valid) continue;
+    if (rows != nullptr) {
+      const float s = __half2float(q.step), z = __half2float(q.low);
+      float back[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        kc[e] = q[e];
-        x[e] = rnd<BF16>(x[e] / kc[e]);
+        back[e] = fmaf(q.code[e], s, z);
+        if (KEY) back[e] *= kd.kc[e];
+        if (!owned) back[e] = 0.f;
       }
+      store_row(rows + ((int64_t)i * p.H + h) * D + c * 8, back);
     }
-    float mn = x[0], mx = x[0];
-#pragma unroll
-    for (int e = 1; e < 8; ++e) {
-      mn = fminf(mn, x[e]);
-      mx = fmaxf(mx, x[e]);
-    }
-#pragma unroll
-    for (int o = 1; o < kGroup / 8; o <<= 1) {
-      mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    }
-    float s = rnd<BF16>(rnd<BF16>(mx - mn) / 15.0f);
-    s = rnd<BF16>(fmaxf(s, 1e-8f));
-    uint32_t packed = 0u;
-    float back[8];
-    const __half sh = __float2half_rn(s), zh = __float2half_rn(mn);
-    const float sf = __half2float(sh), zf = __half2float(zh);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float t = rnd<BF16>(rnd<BF16>(x[e] - mn) / s);
-      const float code = fminf(fmaxf(rintf(t), 0.f), 15.f);
-      packed |= (uint32_t)code << (4 * e);
-      back[e] = fmaf(code, sf, zf);
-      if (key) back[e] *= kc[e];
-    }
-    if (!valid) continue;
-    T* out = reinterpret_cast<T*>(key ? p.k_rows : p.v_rows);
-    if (out != nullptr) {
-      if (!owned) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) back[e] = 0.f;
-      }
-      store8(out + (i * p.H + h) * D + d, back);
-    }
-    if (!owned || slot < 0 || slot >= (int64_t)p.kv.num_pages * p.kv.page_size) continue;
+    if (!owned || slot < 0 || slot >= limit) continue;
     int64_t page, at;
     if (slot <= 0x7fffffffLL) {
-      page = (uint32_t)slot / (uint32_t)p.kv.page_size;
-      at = (uint32_t)slot - (uint32_t)page * (uint32_t)p.kv.page_size;
+      page = p.page_div.div((int)slot);
+      at = slot - page * p.kv.page_size;
     } else {
       page = slot / p.kv.page_size;
       at = slot - page * p.kv.page_size;
     }
-    const int64_t* sq = key ? p.kv.skq : p.kv.svq;
-    const int64_t* sc = key ? p.kv.sks : p.kv.svs;
-    uint8_t* pay = const_cast<uint8_t*>(key ? p.kv.kq : p.kv.vq);
-    *reinterpret_cast<uint32_t*>(pay + page * sq[0] + (int64_t)h * sq[1] + at * sq[2] + c * 4) = packed;
+    *reinterpret_cast<uint32_t*>(pay + page * sq[0] + at * sq[2]) = q.packed;
     if ((c & 3) == 0) {
-      const int64_t o = page * sc[0] + (int64_t)h * sc[1] + at * sc[2] + c / 4;
-      const_cast<uint16_t*>(key ? p.kv.ks : p.kv.vs)[o] = __half_as_ushort(sh);
-      const_cast<uint16_t*>(key ? p.kv.kz : p.kv.vz)[o] = __half_as_ushort(zh);
+      const int64_t o = page * sc[0] + at * sc[2];
+      scale[o] = q.step;
+      zero[o] = q.low;
     }
   }
 }
 
+// grid: (runs of tokens, heads / heads per block, K or V)
 template <typename T, int D>
-int launch(const AppendParams& p, cudaStream_t st) {
-  const int64_t rows = (int64_t)p.N * 2 * p.H;
-  const int64_t per = kThreads / (D / 8);
-  int64_t grid = (rows + per - 1) / per;
-  const int64_t cap = (int64_t)device_sm_count() * 32;
-  if (grid > cap) grid = cap;
-  append_kernel<T, D><<<(int)grid, kThreads, 0, st>>>(p, rows);
+__global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant__ AppendParams p) {
+  constexpr int kLanes = D / 8;                    // threads per row
+  const int c = threadIdx.x % kLanes, row = threadIdx.x / kLanes;
+  const int sub = row / p.heads_per_block, h = blockIdx.y * p.heads_per_block + row - sub * p.heads_per_block;
+  const int step = kThreads / kLanes / p.heads_per_block;
+  const int64_t begin = (int64_t)blockIdx.x * p.run;
+  const int last = (int)min((int64_t)p.N, begin + p.run);
+  const int first = (int)min((int64_t)last, begin + sub);
+  if (blockIdx.z == 0) append_run<T, D, true>(p, first, last, step, h, c);
+  else append_run<T, D, false>(p, first, last, step, h, c);
+}
+
+template <typename T, int D>
+int launch(AppendParams& p, cudaStream_t st) {
+  constexpr int kRows = kThreads / (D / 8);
+  p.heads_per_block = kRows % p.H == 0 ? p.H : 1;
+  const int step = kRows / p.heads_per_block, groups = p.H / p.heads_per_block;
+  // runs of at least one round of the block; at most about 8 blocks an SM over K, V and the heads
+  int64_t runs = ((int64_t)p.N + step - 1) / step;
+  const int64_t cap = ((int64_t)device_sm_count() * 8 + 2 * groups - 1) / (2 * groups);
+  if (runs > cap) runs = cap;
+  const int64_t per = ((int64_t)p.N + runs - 1) / runs;
+  p.run = (int)((per + step - 1) / step * step);
+  runs = ((int64_t)p.N + p.run - 1) / p.run;
+  p.page_div.set((uint32_t)p.kv.page_size);
+  append_kernel<T, D><<<dim3((unsigned)runs, groups, 2), kThreads, 0, st>>>(p);
   return cudaGetLastError() == cudaSuccess ? MA_OK : MA_ERR_CUDA;
 }
 
 }  // namespace
 
-int launch_append_tokens(const AppendParams& p, int dtype, cudaStream_t st) {
+int launch_append_tokens(AppendParams& p, int dtype, cudaStream_t st) {
   if (p.N == 0) return MA_OK;
   if (dtype == MA_BF16) return p.D == 128 ? launch<__nv_bfloat16, 128>(p, st) : launch<__nv_bfloat16, 64>(p, st);
   return p.D == 128 ? launch<float, 128>(p, st) : launch<float, 64>(p, st);

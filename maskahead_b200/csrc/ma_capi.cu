@@ -881,6 +881,7 @@ int ma_append_tokens(const ma_kv* pool, int B, int H, int D, const void* k, cons
                      const int64_t sk[2], const int64_t sv[2], const int64_t* slots, const int32_t* seqs,
                      void* k_rows, void* v_rows, void* stream) {
   if (!pool || B <= 0 || H <= 0 || N < 0) return MA_ERR_ARG;
+  if (H > 65535) return MA_ERR_UNSUPPORTED;
   if (D != 64 && D != 128) return MA_ERR_UNSUPPORTED;
   if (!valid_dtype(dtype)) return MA_ERR_ARG;
   if (pool->layout != MA_KV_PACKED_TOKEN || pool->nf != 0) return MA_ERR_UNSUPPORTED;
@@ -913,9 +914,9 @@ int ma_append_tokens(const ma_kv* pool, int B, int H, int D, const void* k, cons
 
 size_t ma_verify_drafts_workspace(int B, int V) {
   if (B <= 0 || V <= 0) return 0;
-  int chunk, chunks;
-  plan_verify(B, V, chunk, chunks);
-  return 512 + kVerifyTickets * sizeof(unsigned) + (size_t)B * chunks * sizeof(unsigned long long);
+  int span, spans;
+  plan_verify(B, V, span, spans);
+  return 512 + kVerifyTickets * sizeof(unsigned) + (size_t)B * spans * sizeof(unsigned long long);
 }
 
 int ma_verify_drafts(const void* target, const void* draft, int32_t dtype, int B, int K, int V, const int64_t st[2],
@@ -943,7 +944,7 @@ int ma_verify_drafts(const void* target, const void* draft, int32_t dtype, int B
   p.B = B;
   p.K = K;
   p.V = V;
-  plan_verify(B, V, p.chunk, p.chunks);
+  plan_verify(B, V, p.span, p.spans);
   p.accepted = accepted;
   p.out = out;
   char* base = align256(workspace) + 256;

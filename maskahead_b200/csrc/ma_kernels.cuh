@@ -253,8 +253,10 @@ struct AppendParams {
   const int32_t* seqs;
   ma_kv kv;               // the pool (page_size, num_pages; strides over page, head, position)
   void *k_rows, *v_rows;  // [N, H, D] the values the pool now holds, or null
+  int run, heads_per_block;   // set by the launch
+  FastDiv page_div;           // by page_size
 };
-int launch_append_tokens(const AppendParams& p, int dtype, cudaStream_t st);
+int launch_append_tokens(AppendParams& p, int dtype, cudaStream_t st);
 
 // ma_verify.cu: drafted tokens against the target's probabilities
 struct VerifyParams {
@@ -262,12 +264,12 @@ struct VerifyParams {
   int64_t st[2], sd[2];         // strides over (request, position)
   const int32_t *tokens, *counts;
   const float* uniforms;        // [B, K + 1]
-  int B, K, V, chunk, chunks;
+  int B, K, V, span, spans;
   int32_t *accepted, *out;      // [B], [B, K + 1]
   unsigned* tickets;            // [B], zero between calls
-  unsigned long long* sums;     // [B][chunks]
+  unsigned long long* sums;     // [B][spans]
 };
-void plan_verify(int B, int V, int& chunk, int& chunks);
+void plan_verify(int B, int V, int& span, int& spans);
 int verify_max_requests();
 int launch_verify_drafts(const VerifyParams& p, int dtype, cudaStream_t st);
 

@@ -8,8 +8,14 @@
 // numbers do not depend on their order, so the token does not depend on the split.
 //
 // Bound: HBM, one row of p and one of q per request (the other rows are read at one element
-// each). A CTA sums one chunk of one request's row; the last CTA of the request to arrive
-// finds the chunk that holds the threshold and rescans that chunk alone, from L2.
+// each). A warp sums one span of one request's row; the last CTA of the request to arrive
+// finds the span that holds the threshold and rescans that span alone, from L2. The spans make
+// about one wave of CTAs, because every CTA first finds the accepted run for itself (two
+// dependent loads, 1.5 us).
+//
+// floor(r 2^40) takes no conversion (those run at an eighth of the FMA rate): with t = r 2^20 +
+// 2^23 truncated, t's low bits are the upper 20 bits of the weight, and the remainder gives the
+// lower 20 in the same way; the two halves are summed as 32-bit whole numbers.
 #include "ma_kernels.cuh"
 
 namespace ma {
@@ -18,16 +24,24 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kMaxChunks = 1024;
+constexpr int kMaxSpans = 1024;
+constexpr int kMaxSpan = 4096;          // elements: what the last CTA rescans
 constexpr int kMaxRequests = 65535;
+constexpr uint32_t kMagicBits = 0x4B000000u;       // 2^23
 
 __device__ __forceinline__ float value(const float* p, int64_t i) { return __ldg(p + i); }
 __device__ __forceinline__ float value(const __nv_bfloat16* p, int64_t i) { return __bfloat162float(p[i]); }
 __device__ __forceinline__ float value(const __half* p, int64_t i) { return __half2float(p[i]); }
 
-// floor(min(r, 1) 2^40) of a positive r, 0 otherwise (and for NaN)
-__device__ __forceinline__ unsigned long long weight(float r) {
-  return r > 0.f ? __float2ull_rz(fminf(r, 1.f) * 1099511627776.f) : 0ull;
+// The halves of floor(r 2^40), r in [0, 1], each plus the bits of 2^23.
+__device__ __forceinline__ void weight_halves(float r, uint32_t& hi, uint32_t& lo) {
+  const float t = __fmaf_rz(r, 1048576.f, 8388608.f);
+  const float rest = __fmaf_rn(r, 1048576.f, -(t - 8388608.f));      // exact
+  hi = __float_as_uint(t);
+  lo = __float_as_uint(__fmaf_rz(rest, 1048576.f, 8388608.f));
+}
+__device__ __forceinline__ unsigned long long join(uint32_t hi, uint32_t lo, uint32_t n) {
+  return ((unsigned long long)(hi - n * kMagicBits) << 20) + (lo - n * kMagicBits);
 }
 
 __device__ __forceinline__ unsigned long long warp_sum64(unsigned long long v) {
@@ -59,31 +73,86 @@ __device__ __forceinline__ unsigned long long block_scan(unsigned long long v, u
 }
 
 // The row the next token is drawn from: p, and q to subtract (null: nothing; dropped >= 0:
-// a one-hot draft, that token's weight is 0).
+// a one-hot draft, that token's weight is 0). Saturation clamps to [0, 1] and takes NaN to 0.
 template <typename T>
 struct Row {
   const T *p, *q;
   int dropped;
-  __device__ __forceinline__ unsigned long long operator()(int v) const {
+  __device__ __forceinline__ float rest(int v) const {
     const float a = value(p, v);
-    const unsigned long long w = weight(q != nullptr ? a - value(q, v) : a);
-    return v == dropped ? 0ull : w;
+    return __saturatef(q != nullptr ? a - value(q, v) : a);
+  }
+  __device__ __forceinline__ unsigned long long operator()(int v) const {
+    uint32_t hi, lo;
+    weight_halves(rest(v), hi, lo);
+    return v == dropped ? 0ull : join(hi, lo, 1);
+  }
+  // the sum over [begin, end) by one warp: at most kMaxSpan elements, 128 a lane
+  template <bool Q>
+  __device__ __forceinline__ unsigned long long span(int begin, int end) const {
+    const int lane = threadIdx.x & 31;
+    uint32_t hi = 0u, lo = 0u, n = 0u;
+    int v = begin + lane;
+    for (; v + 7 * 32 < end; v += 8 * 32, n += 8) {
+      float a[8], b[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        a[e] = value(p, v + e * 32);
+        b[e] = Q ? value(q, v + e * 32) : 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        uint32_t x, y;
+        weight_halves(__saturatef(a[e] - b[e]), x, y);
+        hi += x;
+        lo += y;
+      }
+    }
+    for (; v < end; v += 32, ++n) {
+      uint32_t x, y;
+      weight_halves(rest(v), x, y);
+      hi += x;
+      lo += y;
+    }
+    unsigned long long s = join(hi, lo, n);
+    if (dropped >= begin && dropped < end && ((dropped - begin) & 31) == lane) {      // the lane that counted it
+      uint32_t x, y;
+      weight_halves(rest(dropped), x, y);
+      s -= join(x, y, 1);
+    }
+    return warp_sum64(s);
+  }
+  __device__ __forceinline__ unsigned long long span(int begin, int end) const {
+    return q != nullptr ? span<true>(begin, end) : span<false>(begin, end);
   }
 };
 
 // The first element of [begin, end) whose inclusive sum (from `before`) is above the mark, by the
-// whole CTA; -1 when there is none. sums: this CTA's shared scratch.
+// whole CTA, kMaxSpan elements at a time; -1 when there is none.
 template <typename T>
 __device__ int find_crossing(const Row<T>& row, int begin, int end, unsigned long long before, unsigned long long mark,
                              unsigned long long* sWarp, int* sFound) {
-  for (int v0 = begin; v0 < end; v0 += kThreads) {
-    const int v = v0 + threadIdx.x;
-    const unsigned long long w = v < end ? row(v) : 0ull;
-    unsigned long long total;
-    const unsigned long long incl = before + block_scan(w, total, sWarp);
+  constexpr int kEach = kMaxSpan / kThreads;
+  for (int v0 = begin; v0 < end; v0 += kMaxSpan) {
+    const int per = min(kEach, (end - v0 + kThreads - 1) / kThreads);       // consecutive elements of a thread
+    unsigned long long w[kEach], mine = 0, total;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      const int v = v0 + threadIdx.x * per + e;
+      w[e] = e < per && v < end ? row(v) : 0ull;
+      mine += w[e];
+    }
+    const unsigned long long incl = before + block_scan(mine, total, sWarp);
     if (threadIdx.x == 0) *sFound = -1;
     __syncthreads();
-    if (incl > mark && incl - w <= mark) *sFound = v;     // exactly one thread
+    if (incl > mark && incl - mine <= mark) {                // exactly one thread
+      unsigned long long at = incl - mine;
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        if (at <= mark && at + w[e] > mark) *sFound = v0 + threadIdx.x * per + e;
+        at += w[e];
+      }
+    }
     __syncthreads();
     const int found = *sFound;
     if (found >= 0) return found;
@@ -100,7 +169,7 @@ __device__ __forceinline__ unsigned long long mark_of(unsigned long long total, 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant__ VerifyParams p) {
   __shared__ unsigned long long sWarp[kWarps];
-  __shared__ int sRun, sLast, sFound, sChunk;
+  __shared__ int sRun, sLast, sFound, sSpan;
   __shared__ unsigned long long sBefore;
   const int b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const T* target = reinterpret_cast<const T*>(p.target) + (int64_t)b * p.st[0];
@@ -134,19 +203,16 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant_
   row.q = run < n && draft != nullptr ? draft + (int64_t)run * p.sd[1] : nullptr;
   row.dropped = run < n && draft == nullptr ? p.tokens[(int64_t)b * p.K + run] : -1;
 
-  const int begin = blockIdx.x * p.chunk, end = min(p.V, begin + p.chunk);
-  unsigned long long sum = 0;
-#pragma unroll 8
-  for (int v = begin + tid; v < end; v += kThreads) sum += row(v);
-  sum = warp_sum64(sum);
-  if (lane == 0) sWarp[warp] = sum;
+  // ---- a span per warp
+  unsigned long long* sums = p.sums + (int64_t)b * p.spans;
+  const int own = blockIdx.x * kWarps + warp;
+  if (own < p.spans) {
+    const unsigned long long sum = row.span(own * p.span, min(p.V, (own + 1) * p.span));
+    if (lane == 0) __stcg(&sums[own], sum);
+  }
+  __threadfence();
   __syncthreads();
-  unsigned long long* sums = p.sums + (int64_t)b * p.chunks;
   if (tid == 0) {
-    sum = 0;
-    for (int w = 0; w < kWarps; ++w) sum += sWarp[w];
-    __stcg(&sums[blockIdx.x], sum);
-    __threadfence();
     sLast = atomicAdd(&p.tickets[b], 1u) == gridDim.x - 1;
     if (sLast) p.tickets[b] = 0u;
   }
@@ -154,12 +220,13 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant_
   if (!sLast) return;
   __threadfence();
 
-  // ---- the request's last CTA: the chunk that holds the threshold, then the token
-  unsigned long long v[kMaxChunks / kThreads], mine = 0, total;
+  // ---- the request's last CTA: the span that holds the threshold, then the token
+  constexpr int kEach = kMaxSpans / kThreads;
+  unsigned long long v[kEach], mine = 0, total;
 #pragma unroll
-  for (int e = 0; e < kMaxChunks / kThreads; ++e) {
-    const int c = tid * (kMaxChunks / kThreads) + e;
-    v[e] = c < p.chunks ? __ldcg(&sums[c]) : 0ull;
+  for (int e = 0; e < kEach; ++e) {
+    const int c = tid * kEach + e;
+    v[e] = c < p.spans ? __ldcg(&sums[c]) : 0ull;
     mine += v[e];
   }
   const unsigned long long incl = block_scan(mine, total, sWarp);
@@ -170,17 +237,16 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant_
     unsigned long long at = incl - mine;
     if (incl > mark && at <= mark) {        // exactly one thread
 #pragma unroll
-      for (int e = 0; e < kMaxChunks / kThreads; ++e) {
+      for (int e = 0; e < kEach; ++e) {
         if (at <= mark && at + v[e] > mark) {
-          sChunk = tid * (kMaxChunks / kThreads) + e;
+          sSpan = tid * kEach + e;
           sBefore = at;
         }
         at += v[e];
       }
     }
     __syncthreads();
-    const int c0 = sChunk * p.chunk;
-    token = find_crossing(row, c0, min(p.V, c0 + p.chunk), sBefore, mark, sWarp, &sFound);
+    token = find_crossing(row, sSpan * p.span, min(p.V, (sSpan + 1) * p.span), sBefore, mark, sWarp, &sFound);
   } else {
     // no residual mass (p <= q everywhere): the row of p itself, read again whole
     row.q = nullptr;
@@ -199,17 +265,20 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant_
 
 int verify_max_requests() { return kMaxRequests; }
 
-// Chunks of a row: enough CTAs for the GPU when there are few requests, long enough that their
-// sums stay few.
-void plan_verify(int B, int V, int& chunk, int& chunks) {
-  chunk = 1024;
-  while (chunk < 8192 && (int64_t)B * ((V + chunk - 1) / chunk) > (int64_t)device_sm_count() * 16) chunk *= 2;
-  while ((V + chunk - 1) / chunk > kMaxChunks) chunk *= 2;
-  chunks = (V + chunk - 1) / chunk;
+// Elements per span: about one wave of CTAs (5 an SM) over all requests, in steps of the 256
+// elements that a warp loads at once; at most kMaxSpans spans a row.
+void plan_verify(int B, int V, int& span, int& spans) {
+  const int64_t warps = (int64_t)device_sm_count() * 5 * kWarps;
+  int64_t n = ((int64_t)B * V + warps - 1) / warps;
+  n = (n + 255) / 256 * 256;
+  if (n > kMaxSpan) n = kMaxSpan;
+  while ((V + n - 1) / n > kMaxSpans) n += 256;
+  span = (int)n;
+  spans = (int)((V + n - 1) / n);
 }
 
 int launch_verify_drafts(const VerifyParams& p, int dtype, cudaStream_t st) {
-  const dim3 grid(p.chunks, p.B);
+  const dim3 grid((p.spans + kWarps - 1) / kWarps, p.B);
   if (dtype == MA_F32) verify_kernel<float><<<grid, kThreads, 0, st>>>(p);
   else if (dtype == MA_BF16) verify_kernel<__nv_bfloat16><<<grid, kThreads, 0, st>>>(p);
   else verify_kernel<__half><<<grid, kThreads, 0, st>>>(p);
