@@ -13,8 +13,9 @@
 // lane. So the bf16 form does without divisions. With 8-bit significands a quotient a / s can
 // neither lie on nor within 2^-17 of a boundary of bf16 rounding (m s = a has no solution for a
 // 9-bit odd m), so a product with a reciprocal that is off by a few ulps rounds to the same
-// bf16. A key's divisor has 24 bits: there the product is checked against the boundary, and the
-// few elements within 4 ulps of it (one in 8000) are divided.
+// bf16. A key's divisor has 24 bits: there two products, with a reciprocal 2^-21 too large and
+// one as much too small, enclose the quotient, and where they round differently (one element
+// in 4000) it is divided.
 #include <type_traits>
 
 #include "ma_kernels.cuh"
@@ -86,61 +87,65 @@ __device__ __forceinline__ Quantized quantize(const uint32_t x[4]) {
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     const uint32_t a = bits(__hsub2(pair(x[e]), low2));
-    float t0, t1;
+    __nv_bfloat162 t;               // in [0, 15.1] or NaN (-> 0)
     if (plain) {
-      t0 = lo_float(a) * rs;
-      t1 = hi_float(a) * rs;
+      t = __hmax2(__floats2bfloat162_rn(lo_float(a) * rs, hi_float(a) * rs), __float2bfloat162_rn(0.f));
     } else {
-      t0 = lo_float(a) / s;
-      t1 = hi_float(a) / s;
+      t = __hmax2(__floats2bfloat162_rn(lo_float(a) / s, hi_float(a) / s), __float2bfloat162_rn(0.f));
+      t = __hmin2(t, __float2bfloat162_rn(15.f));
     }
-    // in [0, 15.1] or NaN (-> 0); 128 + t rounds t to the nearest whole number, ties to even
-    const __nv_bfloat162 t = __hmin2(__hmax2(__floats2bfloat162_rn(t0, t1), __float2bfloat162_rn(0.f)), __float2bfloat162_rn(15.f));
+    // 128 + t rounds t to the nearest whole number, ties to even, and leaves it in the low bits
     c[e] = bits(__hadd2(t, __float2bfloat162_rn(128.f)));
     r.code[2 * e] = lo_float(c[e]) - 128.f;
     r.code[2 * e + 1] = hi_float(c[e]) - 128.f;
-    c[e] = (c[e] & 0xfu) | ((c[e] >> 12) & 0xf0u);
+    c[e] &= 0x000f000fu;
   }
-  r.packed = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+  // (c0, c1), (c2, c3) in 16-bit halves -> four nibbles of a half word
+  const uint32_t u = c[0] + c[1] * 256u, v = c[2] + c[3] * 256u;
+  r.packed = __byte_perm(u | u >> 12, v | v >> 12, 0x5410);
   r.step = __float2half_rn(s);
   r.low = __float2half_rn(low);
   return r;
 }
 
-// A thread's divisors: kc, their reciprocals, and whether the products may be used.
+// A thread's divisors, and for bf16 rows their reciprocals, a little too large and too small.
+template <bool BF16>
 struct Divisors {
-  float kc[8], r[8];
+  float kc[8], above[BF16 ? 8 : 1], below[BF16 ? 8 : 1];
   bool usable;
   __device__ __forceinline__ void load(const float* p) {
     usable = true;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       kc[e] = p[e];
-      r[e] = 1.0f / kc[e];
-      usable &= kc[e] > 1e-30f && kc[e] < 1e30f;
+      if (BF16) {
+        const float r = 1.0f / kc[e];
+        above[e] = r * (1.f + 4.76837158e-7f);
+        below[e] = r * (1.f - 4.76837158e-7f);
+        usable &= kc[e] > 1e-30f && kc[e] < 1e30f;
+      }
     }
   }
 };
 
-__device__ __forceinline__ void divide(const Divisors& k, float x[8]) {
+__device__ __forceinline__ void divide(const Divisors<false>& k, float x[8]) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) x[e] /= k.kc[e];
 }
-__device__ __forceinline__ void divide(const Divisors& k, uint32_t x[4]) {
-  uint32_t near = k.usable ? 0u : 1u;
-  float y[8];
+__device__ __forceinline__ void divide(const Divisors<true>& k, uint32_t x[4]) {
+  uint32_t y[4], apart = k.usable ? 0u : 1u;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    y[e] = ((e & 1) ? hi_float(x[e >> 1]) : lo_float(x[e >> 1])) * k.r[e];
-    // within 4 ulps of a boundary of bf16 rounding (0x8000 in the low half)
-    near |= ((__float_as_uint(y[e]) - 0x7ffcu) & 0xffffu) <= 8u ? 1u : 0u;
+  for (int e = 0; e < 4; ++e) {
+    const float a = lo_float(x[e]), b = hi_float(x[e]);
+    y[e] = bits(__floats2bfloat162_rn(a * k.above[2 * e], b * k.above[2 * e + 1]));
+    apart |= y[e] ^ bits(__floats2bfloat162_rn(a * k.below[2 * e], b * k.below[2 * e + 1]));
   }
-  if (near) {
+  if (apart) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = ((e & 1) ? hi_float(x[e >> 1]) : lo_float(x[e >> 1])) / k.kc[e];
+    for (int e = 0; e < 4; ++e) y[e] = bits(__floats2bfloat162_rn(lo_float(x[e]) / k.kc[2 * e], hi_float(x[e]) / k.kc[2 * e + 1]));
   }
 #pragma unroll
-  for (int e = 0; e < 4; ++e) x[e] = bits(__floats2bfloat162_rn(y[2 * e], y[2 * e + 1]));
+  for (int e = 0; e < 4; ++e) x[e] = y[e];
 }
 
 __device__ __forceinline__ void load_row(const float* p, float x[8]) { load8(p, x); }
@@ -171,7 +176,7 @@ __device__ __forceinline__ void append_run(const AppendParams& p, int first, int
   __half* zero = reinterpret_cast<__half*>(const_cast<uint16_t*>(KEY ? p.kv.kz : p.kv.vz)) + sc0;
   const int64_t limit = (int64_t)p.kv.num_pages * p.kv.page_size;
 
-  Divisors kd;
+  Divisors<sizeof(T) == 2> kd;
   int held = -2;          // the request whose divisors are in kd
   Raw next[kRaw] = {};
   int64_t next_slot = -1;

@@ -240,9 +240,10 @@ struct PagePlanParams {
   int32_t *seqs, *positions;
   unsigned* ticket;
   int pages_in_place, free_in_place;
+  FastDiv page_div;   // by page_size, set by the launch
 };
 int page_plan_max_requests();
-int launch_page_plan(const PagePlanParams& p, cudaStream_t st);
+int launch_page_plan(PagePlanParams& p, cudaStream_t st);
 
 // ma_append.cu: K/V rows of new tokens quantized into the slots of a packed pool
 struct AppendParams {

@@ -22,34 +22,41 @@ constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxRequests = 8192;
 
-__device__ __forceinline__ int pages_of(int len, int page) { return len / page + (len % page != 0); }
+// a + b, or the largest value: sums only have to be right up to the limits they are held to
+__device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) {
+  const uint32_t s = a + b;
+  return s < a ? 0xffffffffu : s;
+}
 
-// Inclusive scan over the CTA of three sums at once; total[] = the CTA's sums.
-__device__ __forceinline__ void block_scan3(long long v[3], long long total[3], long long (*sWarp)[kWarps]) {
+// Exclusive saturating scan over the CTA of three sums at once; total[] = the CTA's sums.
+__device__ __forceinline__ void block_scan3(uint32_t v[3], uint32_t total[3], uint32_t (*sWarp)[kWarps]) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint32_t incl[3];
 #pragma unroll
   for (int k = 0; k < 3; ++k) {
+    incl[k] = v[k];
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long u = __shfl_up_sync(0xffffffffu, v[k], o);
-      if (lane >= o) v[k] += u;
+      const uint32_t u = __shfl_up_sync(0xffffffffu, incl[k], o);
+      if (lane >= o) incl[k] = add_sat(incl[k], u);
     }
-    if (lane == 31) sWarp[k][warp] = v[k];
+    if (lane == 31) sWarp[k][warp] = incl[k];
   }
   __syncthreads();
 #pragma unroll
-  for (int k = 0; k < 3; ++k) {
-    long long before = 0, sum = 0;
+  for (int k = 0; k < 3; ++k) {           // every warp scans the warps' sums for itself
+    uint32_t u = lane < kWarps ? sWarp[k][lane] : 0u;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const long long u = sWarp[k][w];
-      if (w < warp) before += u;
-      sum += u;
+    for (int o = 1; o < kWarps; o <<= 1) {
+      const uint32_t x = __shfl_up_sync(0xffffffffu, u, o);
+      if (lane >= o) u = add_sat(u, x);
     }
-    v[k] += before;
-    total[k] = sum;
+    total[k] = __shfl_sync(0xffffffffu, u, kWarps - 1);
+    const uint32_t before = __shfl_sync(0xffffffffu, u, warp > 0 ? warp - 1 : 0);
+    uint32_t lower = __shfl_up_sync(0xffffffffu, incl[k], 1);
+    if (lane == 0) lower = 0u;
+    v[k] = warp > 0 ? add_sat(lower, before) : lower;
   }
-  __syncthreads();
 }
 
 // The last b in [0, n) with start[b] <= x (start ascending, start[0] = 0 <= x).
@@ -65,9 +72,9 @@ __device__ __forceinline__ int owner_of(const int* start, int n, int x) {
 
 __global__ void __launch_bounds__(kThreads) page_plan_kernel(const __grid_constant__ PagePlanParams p) {
   extern __shared__ int sMem[];
-  __shared__ long long sWarp[3][kWarps];
+  __shared__ uint32_t sWarp[3][kWarps];
   __shared__ int sLast;
-  const int tid = threadIdx.x, B = p.B;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, B = p.B;
   // [B + 1] first new token, first taken page, first returned page of each request; [B] old
   // length and wanted length
   int* sTok = sMem;
@@ -75,60 +82,70 @@ __global__ void __launch_bounds__(kThreads) page_plan_kernel(const __grid_consta
   int* sGive = sTake + B + 1;
   int* sLen = sGive + B + 1;
   int* sWant = sLen + B;
+  auto pages_of = [&](int len) { return len > 0 ? p.page_div.div(len - 1) + 1 : 0; };
 
   const int count = min(max(*p.free_count, 0), p.num_pages);
   const int64_t most = (int64_t)p.width * p.page_size;      // a length past its table is the table's
   const int longest = most < 0x7fffffffLL ? (int)most : 0x7fffffff;
-  long long given = 0;                      // pages handed back by all requests
-  for (int b = tid; b < B; b += kThreads) {
+  // ---- the sums of all requests as they ask: pages needed and tokens (saturating), pages
+  // returned. A thread has `each` neighbouring requests.
+  const int each = (B + kThreads - 1) / kThreads, b_lo = min(B, tid * each), b_hi = min(B, b_lo + each);
+  uint32_t v[3] = {0u, 0u, 0u}, total[3];
+  for (int b = b_lo; b < b_hi; ++b) {
     const int len = min(max(p.lens[b], 0), longest);
     int want = max(p.new_lens[b], 0);
-    if (pages_of(want, p.page_size) > p.width) want = len;      // longer than the table: stays as it is
+    if (want > longest) want = len;        // longer than the table: stays as it is
     sLen[b] = len;
     sWant[b] = want;
-    given += max(pages_of(len, p.page_size) - pages_of(want, p.page_size), 0);
+    const int had = pages_of(len), get = pages_of(want);
+    v[0] = add_sat(v[0], max(get - had, 0));
+    v[1] = add_sat(v[1], max(want - len, 0));
+    sGive[b] = (int)v[2];
+    v[2] += max(had - get, 0);
+    sTake[b] = (int)v[0];                  // inclusive sums of the thread's own requests, for now
+    sTok[b] = (int)v[1];
   }
-  {
-    long long v[3] = {given, 0, 0}, total[3];
-    block_scan3(v, total, sWarp);
-    given = total[0];
-  }
-  const long long avail = count + given;
-  long long need0 = 0, tok0 = 0, give0 = 0, need_ok = 0, tok_ok = 0;
-  for (int b0 = 0; b0 < B; b0 += kThreads) {
-    const int b = b0 + tid;
-    const int len = b < B ? sLen[b] : 0, want = b < B ? sWant[b] : 0;
-    const int had = pages_of(len, p.page_size), get = pages_of(want, p.page_size);
-    long long v[3] = {max(get - had, 0), max(want - len, 0), max(had - get, 0)}, total[3];
-    const long long need = v[0], tok = v[1], give = v[2];
-    block_scan3(v, total, sWarp);
-    // the sums only grow: once one is too large no later request fits
-    const bool fits = need0 + v[0] <= avail && tok0 + v[1] <= p.max_tokens;
-    // exclusive sums over the granted requests: the raw ones while they fit, the last fitting
-    // ones from then on
-    long long ok[3] = {fits ? need : 0, fits ? tok : 0, 0}, okt[3];
-    block_scan3(ok, okt, sWarp);
-    if (b < B) {
-      sTake[b] = (int)(need_ok + ok[0] - (fits ? need : 0));
-      sTok[b] = (int)(tok_ok + ok[1] - (fits ? tok : 0));
-      sGive[b] = (int)(give0 + v[2] - give);
-      if (!fits && want > len) sWant[b] = len;
+  block_scan3(v, total, sWarp);
+  const uint32_t give0 = total[2];
+  // ---- grants: the sums only grow, so the requests that fit are the first ones; behind the last of
+  // them the sums stay
+  const uint32_t avail = (uint32_t)count + give0;
+  uint32_t taken = 0u, tokens = 0u;
+  for (int b = b_lo; b < b_hi; ++b) {
+    const uint32_t need = add_sat(v[0], (uint32_t)sTake[b]), tok = add_sat(v[1], (uint32_t)sTok[b]);
+    sTake[b] = (int)need;
+    sTok[b] = (int)tok;
+    sGive[b] += (int)v[2];
+    if (need <= avail && tok <= (uint32_t)p.max_tokens) {
+      taken = need;
+      tokens = tok;
     }
-    need0 += total[0];
-    tok0 += total[1];
-    give0 += total[2];
-    need_ok += okt[0];
-    tok_ok += okt[1];
   }
-  const int taken = (int)need_ok, tokens = (int)tok_ok, back = (int)give0;
+  __syncthreads();                         // the scan's sums are read
+  taken = __reduce_max_sync(0xffffffffu, taken);
+  tokens = __reduce_max_sync(0xffffffffu, tokens);
+  if (lane == 0) {
+    sWarp[0][warp] = taken;
+    sWarp[1][warp] = tokens;
+  }
+  __syncthreads();
+  taken = __reduce_max_sync(0xffffffffu, lane < kWarps ? sWarp[0][lane] : 0u);
+  tokens = __reduce_max_sync(0xffffffffu, lane < kWarps ? sWarp[1][lane] : 0u);
+  for (int b = b_lo; b < b_hi; ++b) {             // exclusive sums of what is granted
+    const int len = sLen[b], want = sWant[b];
+    const bool fits = (uint32_t)sTake[b] <= avail && (uint32_t)sTok[b] <= (uint32_t)p.max_tokens;
+    sTake[b] = fits ? sTake[b] - max(pages_of(want) - pages_of(len), 0) : (int)taken;
+    sTok[b] = fits ? sTok[b] - max(want - len, 0) : (int)tokens;
+    if (!fits && want > len) sWant[b] = len;
+  }
   if (tid == 0) {
-    sTake[B] = taken;
-    sTok[B] = tokens;
-    sGive[B] = back;
+    sTake[B] = (int)taken;
+    sTok[B] = (int)tokens;
+    sGive[B] = (int)give0;
   }
   // (a table that gives back more pages than the pool has lost is the caller's error: the count
   // stops at the pool's size)
-  const int top = count + back, left = min(top - taken, p.num_pages);
+  const int top = count + (int)give0, left = min(top - (int)taken, p.num_pages);
   __syncthreads();                           // every length of this CTA's copy is read and granted
 
   if (tid == 0) {
@@ -153,7 +170,7 @@ __global__ void __launch_bounds__(kThreads) page_plan_kernel(const __grid_consta
     if (i < count) return p.free_list[i];
     const int r = i - count;
     const int b = owner_of(sGive, B, r);
-    return p.pages[(int64_t)b * p.spg + pages_of(sWant[b], p.page_size) + (r - sGive[b])];
+    return p.pages[(int64_t)b * p.spg + pages_of(sWant[b]) + (r - sGive[b])];
   };
   auto taken_page = [&](int b, int k) -> int { return stacked(top - 1 - (sTake[b] + k)); };
 
@@ -161,33 +178,57 @@ __global__ void __launch_bounds__(kThreads) page_plan_kernel(const __grid_consta
 
   // ---- the tokens, four to a thread
   const int64_t quads = ((int64_t)p.max_tokens + 3) / 4;
+  int b = -1;
   for (int64_t qd = first; qd < quads; qd += step) {
     const int i0 = (int)(qd * 4);
     long long slot[4];
     int own[4], pos[4];
-    int b = -1, page = -1, at = -1, off = 0;
+    // requests without tokens share their start with the next: the owner is the last one at or below
+    if (i0 < (int)tokens && (b < 0 || i0 >= sTok[b + 1])) b = owner_of(sTok, B, i0);
+    auto page_at = [&](int at) {
+      const int had = pages_of(sLen[b]);
+      const int page = at < had ? p.pages[(int64_t)b * p.spg + at] : taken_page(b, at - had);
+      return page >= 0 && page < p.num_pages ? page : -1;
+    };
+    const int x0 = i0 < (int)tokens ? sLen[b] + (i0 - sTok[b]) : 0;
+    int at = p.page_div.div(x0), off = x0 - at * p.page_size;
+    if (i0 < (int)tokens && i0 + 3 < sTok[b + 1] && p.page_size >= 4) {
+      // one request, at most two pages (some lane of a warp crosses one in most rounds)
+      const int page = page_at(at), left_here = p.page_size - off;
+      const int after = left_here < 4 ? page_at(at + 1) : -1;
+      const long long here = page >= 0 ? (long long)page * p.page_size + off : -1ll;
+      const long long there = after >= 0 ? (long long)after * p.page_size - left_here : -1ll;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int i = i0 + e;
-      slot[e] = -1;
-      own[e] = pos[e] = -1;
-      if (i >= tokens) continue;
-      if (b < 0 || i >= sTok[b + 1]) {
-        // requests without tokens share their start with the next: the last one at or below i
-        b = b < 0 ? owner_of(sTok, B, i) : b + 1;
-        while (i >= sTok[b + 1]) ++b;
-        at = -1;
+      for (int e = 0; e < 4; ++e) {
+        slot[e] = e < left_here ? (page >= 0 ? here + e : -1ll) : (after >= 0 ? there + e : -1ll);
+        own[e] = b;
+        pos[e] = x0 + e;
       }
-      const int x = sLen[b] + (i - sTok[b]);
-      if (at < 0 || ++off == p.page_size) {
-        at = x / p.page_size;
-        off = x - at * p.page_size;
-        const int had = pages_of(sLen[b], p.page_size);
-        page = at < had ? p.pages[(int64_t)b * p.spg + at] : taken_page(b, at - had);
+    } else {
+      int page = -2;
+#pragma unroll 1
+      for (int e = 0; e < 4; ++e) {
+        const int i = i0 + e;
+        long long s = -1;
+        int o = -1, x = -1;
+        if (i < (int)tokens) {
+          if (i >= sTok[b + 1]) {
+            do ++b; while (i >= sTok[b + 1]);
+            page = -2;
+          }
+          x = sLen[b] + (i - sTok[b]);
+          at = p.page_div.div(x);
+          off = x - at * p.page_size;
+          if (page == -2 || off == 0) page = page_at(at);
+          o = b;
+          if (page >= 0) s = (long long)page * p.page_size + off;
+        }
+        // (registers, not local memory: no dynamic index)
+        if (e == 0) { slot[0] = s; own[0] = o; pos[0] = x; }
+        else if (e == 1) { slot[1] = s; own[1] = o; pos[1] = x; }
+        else if (e == 2) { slot[2] = s; own[2] = o; pos[2] = x; }
+        else { slot[3] = s; own[3] = o; pos[3] = x; }
       }
-      own[e] = b;
-      pos[e] = x;
-      if (page >= 0 && page < p.num_pages) slot[e] = (long long)page * p.page_size + off;
     }
     if (i0 + 4 <= p.max_tokens) {
       reinterpret_cast<longlong2*>(p.slots + i0)[0] = make_longlong2(slot[0], slot[1]);
@@ -205,22 +246,18 @@ __global__ void __launch_bounds__(kThreads) page_plan_kernel(const __grid_consta
     }
   }
 
-  // ---- the page table. In place only the taken pages are written; returned entries keep their
-  // stale number behind the length, so nothing that is read here is written here.
-  if (p.pages_in_place) {
-    for (int64_t i = first; i < taken; i += step) {
-      const int b = owner_of(sTake, B, (int)i);
-      const int k = (int)i - sTake[b];
-      p.pages_out[(int64_t)b * p.spg_out + pages_of(sLen[b], p.page_size) + k] = taken_page(b, k);
-    }
-  } else {
-    const int64_t entries = (int64_t)B * p.width;
-    for (int64_t i = first; i < entries; i += step) {
-      const int b = (int)(i / p.width), j = (int)(i - (int64_t)b * p.width);
-      const int k = j - pages_of(sLen[b], p.page_size);
-      p.pages_out[(int64_t)b * p.spg_out + j] =
-          k >= 0 && k < sTake[b + 1] - sTake[b] ? taken_page(b, k) : p.pages[(int64_t)b * p.spg + j];
-    }
+  // ---- the page table, 32 entries of a request per warp and round. In place only the taken pages
+  // are written; returned entries keep their stale number behind the length, so nothing that is
+  // read here is written here.
+  const int warps = gridDim.x * kWarps, pieces = (p.width + 31) / 32;
+  for (int64_t u = blockIdx.x * kWarps + warp; u < (int64_t)B * pieces; u += warps) {
+    const int r = (int)(u / pieces), j0 = (int)(u - (int64_t)r * pieces) * 32;
+    const int had = pages_of(sLen[r]), taken_r = sTake[r + 1] - sTake[r];
+    if (p.pages_in_place && (j0 + 32 <= had || j0 >= had + taken_r)) continue;
+    const int j = j0 + lane, k = j - had;
+    if (j >= p.width) continue;
+    if (k >= 0 && k < taken_r) p.pages_out[(int64_t)r * p.spg_out + j] = taken_page(r, k);
+    else if (!p.pages_in_place) p.pages_out[(int64_t)r * p.spg_out + j] = p.pages[(int64_t)r * p.spg + j];
   }
 
   // ---- the free stack: the returned pages that were not taken again
@@ -236,16 +273,17 @@ __global__ void __launch_bounds__(kThreads) page_plan_kernel(const __grid_consta
 
 int page_plan_max_requests() { return kMaxRequests; }
 
-int launch_page_plan(const PagePlanParams& p, cudaStream_t st) {
+int launch_page_plan(PagePlanParams& p, cudaStream_t st) {
   const size_t smem = (5 * (size_t)p.B + 3) * sizeof(int);
-  if (cudaFuncSetAttribute(page_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 5 * (kMaxRequests + 1) * (int)sizeof(int)) !=
-      cudaSuccess)
+  if (smem > 48 * 1024 &&
+      cudaFuncSetAttribute(page_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
     return MA_ERR_CUDA;
   int64_t items = ((int64_t)p.max_tokens + 3) / 4;
   if (!p.pages_in_place) items = items > (int64_t)p.B * p.width ? items : (int64_t)p.B * p.width;
   if (!p.free_in_place) items = items > p.num_pages ? items : p.num_pages;
   int64_t grid = (items + kThreads - 1) / kThreads;
   const int64_t cap = (int64_t)device_sm_count() * (p.B <= 1024 ? 2 : 1);
+  p.page_div.set((uint32_t)p.page_size);
   grid = grid < 1 ? 1 : grid > cap ? cap : grid;
   page_plan_kernel<<<(int)grid, kThreads, smem, st>>>(p);
   return cudaGetLastError() == cudaSuccess ? MA_OK : MA_ERR_CUDA;
