@@ -468,12 +468,25 @@ MA_API int ma_prefix_attention_gather(const ma_rows* q, const ma_kv* kv, int H, 
  *   inclusive sum exceeds floor(U sum(w) / 2^24) -- whole numbers, so the same token whatever
  *   the order of the sums; -1 if p_a has no mass. out [B, K + 1]: the accepted drafts, the
  *   next token, then -1. V above 2^20 or B above 65535 returns MA_ERR_UNSUPPORTED.       */
+typedef struct ma_page_plan_args {
+  const int32_t* lens;        /* [B] */
+  const int32_t* pages;       /* [B, width], row stride spg */
+  const int32_t* free_list;   /* [num_pages] */
+  const int32_t* free_count;  /* [1] */
+  int32_t B, width, num_pages, page_size, max_tokens;
+  int64_t spg, spg_out;
+  int32_t* lens_out;          /* outputs: see above */
+  int32_t* pages_out;
+  int32_t* free_out;
+  int32_t* free_count_out;
+  int32_t* starts;
+  int64_t* slots;
+  int32_t* seqs;
+  int32_t* positions;
+} ma_page_plan_args;
 MA_API size_t ma_page_plan_workspace(void);
-MA_API int ma_page_plan(const int32_t* lens, const int32_t* new_lens, int B, const int32_t* pages, int64_t spg,
-                        int width, const int32_t* free_list, const int32_t* free_count, int num_pages, int page_size,
-                        int max_tokens, int32_t* lens_out, int32_t* pages_out, int64_t spg_out, int32_t* free_out,
-                        int32_t* free_count_out, int32_t* starts, int64_t* slots, int32_t* seqs, int32_t* positions,
-                        void* workspace, size_t workspace_bytes, void* stream);
+MA_API int ma_page_plan(const ma_page_plan_args* a, const int32_t* new_lens, void* workspace, size_t workspace_bytes,
+                        void* stream);
 MA_API int ma_append_tokens(const ma_kv* pool, int B, int H, int D, const void* k, const void* v, int32_t dtype, int N,
                             const int64_t sk[2], const int64_t sv[2], const int64_t* slots, const int32_t* seqs,
                             void* k_rows, void* v_rows, void* stream);

@@ -68,6 +68,19 @@ class MaBlock(ctypes.Structure):
     ]
 
 
+class MaPagePlan(ctypes.Structure):
+    _fields_ = [
+        ("lens", ctypes.c_void_p), ("pages", ctypes.c_void_p), ("free_list", ctypes.c_void_p),
+        ("free_count", ctypes.c_void_p),
+        ("B", ctypes.c_int32), ("width", ctypes.c_int32), ("num_pages", ctypes.c_int32),
+        ("page_size", ctypes.c_int32), ("max_tokens", ctypes.c_int32),
+        ("spg", ctypes.c_int64), ("spg_out", ctypes.c_int64),
+        ("lens_out", ctypes.c_void_p), ("pages_out", ctypes.c_void_p), ("free_out", ctypes.c_void_p),
+        ("free_count_out", ctypes.c_void_p), ("starts", ctypes.c_void_p), ("slots", ctypes.c_void_p),
+        ("seqs", ctypes.c_void_p), ("positions", ctypes.c_void_p),
+    ]
+
+
 _P = ctypes.POINTER
 _vp, _i32, _f32, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_size_t
 
@@ -125,8 +138,7 @@ _SIGNATURES = {
                                           _vp, _P(ctypes.c_int64), _vp, _vp, _vp, _vp, _sz, _i32, _i32, _P(_vp),
                                           _i32, _vp, _P(ctypes.c_int64), _vp, _sz, _vp]),
     "ma_page_plan_workspace": (_sz, []),
-    "ma_page_plan": (_i32, [_vp, _vp, _i32, _vp, ctypes.c_int64, _i32, _vp, _vp, _i32, _i32, _i32, _vp, _vp,
-                            ctypes.c_int64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "ma_page_plan": (_i32, [_P(MaPagePlan), _vp, _vp, _sz, _vp]),
     "ma_append_tokens": (_i32, [_P(MaKV), _i32, _i32, _i32, _vp, _vp, _i32, _i32, _P(ctypes.c_int64),
                                 _P(ctypes.c_int64), _vp, _vp, _vp, _vp, _vp]),
     "ma_decode_attention_workspace": (_sz, [_i32] * 5),

@@ -836,44 +836,42 @@ int ma_decode_attention(const ma_rows* q, const ma_kv* kv, int H, const ma_block
 
 size_t ma_page_plan_workspace(void) { return 512; }
 
-int ma_page_plan(const int32_t* lens, const int32_t* new_lens, int B, const int32_t* pages, int64_t spg, int width,
-                 const int32_t* free_list, const int32_t* free_count, int num_pages, int page_size, int max_tokens,
-                 int32_t* lens_out, int32_t* pages_out, int64_t spg_out, int32_t* free_out, int32_t* free_count_out,
-                 int32_t* starts, int64_t* slots, int32_t* seqs, int32_t* positions, void* workspace,
-                 size_t workspace_bytes, void* stream) {
-  if (B <= 0 || width <= 0 || num_pages <= 0 || page_size <= 0 || max_tokens < 0) return MA_ERR_ARG;
-  if (!lens || !new_lens || !pages || !free_list || !free_count || !lens_out || !pages_out || !free_out ||
-      !free_count_out || !starts)
+int ma_page_plan(const ma_page_plan_args* a, const int32_t* new_lens, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!a || !new_lens || a->B <= 0 || a->width <= 0 || a->num_pages <= 0 || a->page_size <= 0 || a->max_tokens < 0)
     return MA_ERR_ARG;
-  if (max_tokens > 0 && (!slots || !seqs || !positions || !aligned16(slots) || !aligned16(seqs) || !aligned16(positions)))
+  if (!a->lens || !a->pages || !a->free_list || !a->free_count || !a->lens_out || !a->pages_out || !a->free_out ||
+      !a->free_count_out || !a->starts)
     return MA_ERR_ARG;
-  if (spg < width || spg_out < width || (pages == pages_out && spg != spg_out)) return MA_ERR_ARG;
-  if (B > page_plan_max_requests() || (int64_t)B * width > 0x7fffffffLL) return MA_ERR_UNSUPPORTED;
+  if (a->max_tokens > 0 && (!a->slots || !a->seqs || !a->positions || !aligned16(a->slots) || !aligned16(a->seqs) ||
+                            !aligned16(a->positions)))
+    return MA_ERR_ARG;
+  if (a->spg < a->width || a->spg_out < a->width || (a->pages == a->pages_out && a->spg != a->spg_out)) return MA_ERR_ARG;
+  if (a->B > page_plan_max_requests() || (int64_t)a->B * a->width > 0x7fffffffLL) return MA_ERR_UNSUPPORTED;
   if (!workspace || workspace_bytes < ma_page_plan_workspace()) return MA_ERR_WORKSPACE;
   PagePlanParams p;
-  p.lens = lens;
+  p.lens = a->lens;
   p.new_lens = new_lens;
-  p.pages = pages;
-  p.free_list = free_list;
-  p.free_count = free_count;
-  p.B = B;
-  p.width = width;
-  p.num_pages = num_pages;
-  p.page_size = page_size;
-  p.max_tokens = max_tokens;
-  p.spg = spg;
-  p.spg_out = spg_out;
-  p.lens_out = lens_out;
-  p.pages_out = pages_out;
-  p.free_out = free_out;
-  p.count_out = free_count_out;
-  p.starts = starts;
-  p.slots = slots;
-  p.seqs = seqs;
-  p.positions = positions;
+  p.pages = a->pages;
+  p.free_list = a->free_list;
+  p.free_count = a->free_count;
+  p.B = a->B;
+  p.width = a->width;
+  p.num_pages = a->num_pages;
+  p.page_size = a->page_size;
+  p.max_tokens = a->max_tokens;
+  p.spg = a->spg;
+  p.spg_out = a->spg_out;
+  p.lens_out = a->lens_out;
+  p.pages_out = a->pages_out;
+  p.free_out = a->free_out;
+  p.count_out = a->free_count_out;
+  p.starts = a->starts;
+  p.slots = a->slots;
+  p.seqs = a->seqs;
+  p.positions = a->positions;
   p.ticket = reinterpret_cast<unsigned*>(align256(workspace) + 128);
-  p.pages_in_place = pages == pages_out ? 1 : 0;
-  p.free_in_place = free_list == free_out ? 1 : 0;
+  p.pages_in_place = a->pages == a->pages_out ? 1 : 0;
+  p.free_in_place = a->free_list == a->free_out ? 1 : 0;
   return launch_page_plan(p, (cudaStream_t)stream);
 }
 

@@ -43,12 +43,20 @@ MAX_DECODE_ROWS = 64
 _GROUP = 32
 
 
-def _workspace(device: torch.device, purpose: str, nbytes: int, given: torch.Tensor | None) -> torch.Tensor:
+_SHARED: dict[tuple, tuple] = {}     # (device index, purpose) -> (the shared workspace, its address, its bytes)
+
+
+def _scratch(device: torch.device, purpose: str, nbytes: int, given: torch.Tensor | None) -> tuple[int, int]:
+    """(address, bytes) of a call's workspace: the caller's, or the shared one of the device."""
     if given is None:
-        return _lib.workspace(device, purpose, nbytes)
-    if given.dtype != torch.uint8 or not given.is_contiguous() or given.device != device or given.numel() < nbytes:
+        held = _SHARED.get((device.index, purpose))
+        if held is None or held[2] < nbytes:       # (the shared workspace of a purpose only ever grows, and only here)
+            ws = _lib.workspace(device, purpose, nbytes)
+            held = _SHARED[(device.index, purpose)] = (ws, ws.data_ptr(), ws.numel())
+        return held[1], held[2]
+    if (given.dtype != torch.uint8 or not given.is_contiguous() or given.device != device or given.numel() < nbytes):
         raise ValueError(f"workspace: need a contiguous uint8 tensor of at least {nbytes} bytes on {device}")
-    return given
+    return given.data_ptr(), given.numel()
 
 
 def decode_workspace_bytes(batch: int, heads: int, rows: int, head_dim: int, block_tokens: int = 0) -> int:
@@ -113,18 +121,21 @@ class TokenPlan:
         self.seqs = torch.empty(max_tokens, device=dev, dtype=torch.int32)
         self.positions = torch.empty(max_tokens, device=dev, dtype=torch.int32)
         self._call = _lib.lib().ma_page_plan
-        self._a = (b, pages.data_ptr(), pages.stride(0) if b > 1 else width, width, free.data_ptr(),
-                   free_count.data_ptr(), self.num_pages, self.page_size, self.max_tokens, self.lens.data_ptr(),
-                   self.pages.data_ptr(), self.pages.stride(0) if b > 1 else width, self.free.data_ptr(),
-                   self.free_count.data_ptr(), self.starts.data_ptr(), self.slots.data_ptr(), self.seqs.data_ptr(),
-                   self.positions.data_ptr())
+        self._index = lens.get_device()
+        self._args = _lib.MaPagePlan(
+            lens.data_ptr(), pages.data_ptr(), free.data_ptr(), free_count.data_ptr(), b, width, self.num_pages,
+            self.page_size, self.max_tokens, pages.stride(0) if b > 1 else width,
+            self.pages.stride(0) if b > 1 else width, self.lens.data_ptr(), self.pages.data_ptr(), self.free.data_ptr(),
+            self.free_count.data_ptr(), self.starts.data_ptr(), self.slots.data_ptr(), self.seqs.data_ptr(),
+            self.positions.data_ptr())
 
     def build(self, new_lens: torch.Tensor, *, workspace: torch.Tensor | None = None) -> "TokenPlan":
         """Plan the step whose requests shall have new_lens [B] int32 tokens; returns self."""
-        _check("new_lens", new_lens, torch.int32, (self.batch,), self.device)
-        ws = _workspace(self.device, "page_plan", PLAN_WORKSPACE_BYTES, workspace)
-        rc = self._call(self._in[0].data_ptr(), new_lens.data_ptr(), *self._a, ws.data_ptr(), ws.numel(),
-                        _lib.stream_handle(self.device))
+        if (new_lens.dtype is not torch.int32 or new_lens.get_device() != self._index or new_lens.dim() != 1
+                or new_lens.size(0) != self.batch or not new_lens.is_contiguous()):
+            _check("new_lens", new_lens, torch.int32, (self.batch,), self.device)
+        ws = _scratch(self.device, "page_plan", PLAN_WORKSPACE_BYTES, workspace)
+        rc = self._call(self._args, new_lens.data_ptr(), *ws, _lib.stream_handle(self.device))
         if rc:
             _lib.check("ma_page_plan", rc)
         return self
@@ -157,6 +168,7 @@ class PagedCache:
         if tuple(kchan.shape) != (self.batch, self.heads, self.head_dim):
             raise ValueError(f"kchan must be [B, H, D] = {(self.batch, self.heads, self.head_dim)}")
         self.device = kq.device
+        self._index = kq.get_device()
         for t in (ks, kz, vq, vs, vz, kchan, pages, lens):
             if t.device != self.device:
                 raise ValueError("a cache's tensors must lie on one device")
@@ -198,27 +210,41 @@ class PagedCache:
         divided by the divisor of request seqs[i] (int32). The bytes are those of
         layouts.quantize_tokens. return_rows: also the values the slots now stand for, (k, v)
         [N, H, D] in the rows' type."""
-        if key.ndim != 3 or key.shape != value.shape or key.dtype != value.dtype:
-            raise ValueError("key and value must be [N, H, D] tensors of one shape and type")
-        n, heads, dim = key.shape
-        dev = self.device
-        if heads != self.heads or dim != self.head_dim:
-            raise ValueError(f"rows must be [N, {self.heads}, {self.head_dim}]")
-        if key.device != dev or value.device != dev:
-            raise ValueError(f"rows must lie on {dev}")
-        _check("slots", slots, torch.int64, (n,), dev)
-        _check("seqs", seqs, torch.int32, (n,), dev)
-        k, v = _aligned(key), _aligned(value)
+        shape, index, dev = key.shape, self._index, self.device
+        n = shape[0] if len(shape) == 3 else -1
+        if (n < 0 or value.shape != shape or value.dtype is not key.dtype or shape[1] != self.heads
+                or shape[2] != self.head_dim or key.get_device() != index or value.get_device() != index
+                or slots.dtype is not torch.int64 or slots.shape != (n,) or slots.get_device() != index
+                or seqs.dtype is not torch.int32 or seqs.shape != (n,) or seqs.get_device() != index
+                or not slots.is_contiguous() or not seqs.is_contiguous()):
+            self._refuse_append(key, value, slots, seqs)
+        code = _lib.dtype_code(key.dtype)
+        k, v = key, value
+        if not (k.is_contiguous() and v.is_contiguous()) or (k.data_ptr() | v.data_ptr()) & 15:
+            k, v = _aligned(k), _aligned(v)
         rows_k = rows_v = None
         if return_rows:
-            rows_k, rows_v = torch.empty((2, n, heads, dim), device=dev, dtype=key.dtype).unbind(0)
+            rows_k = torch.empty_like(k) if k.is_contiguous() else k.new_empty(shape)
+            rows_v = torch.empty_like(rows_k)
         rc = self._lib.ma_append_tokens(
-            self._desc.kv, self.batch, heads, dim, k.data_ptr(), v.data_ptr(), _lib.dtype_code(key.dtype), n,
-            _strides(k.stride()[:2]), _strides(v.stride()[:2]), slots.data_ptr(), seqs.data_ptr(), _lib.ptr(rows_k),
-            _lib.ptr(rows_v), _lib.stream_handle(dev))
+            self._desc.kv, self.batch, self.heads, self.head_dim, k.data_ptr(), v.data_ptr(), code, n,
+            _strides(k.stride()[:2]), _strides(v.stride()[:2]), slots.data_ptr(), seqs.data_ptr(),
+            rows_k.data_ptr() if return_rows else None, rows_v.data_ptr() if return_rows else None,
+            _lib.stream_handle(dev))
         if rc:
             _lib.check("ma_append_tokens", rc)
         return (rows_k, rows_v) if return_rows else None
+
+    def _refuse_append(self, key, value, slots, seqs) -> None:
+        if key.ndim != 3 or key.shape != value.shape or key.dtype != value.dtype:
+            raise ValueError("key and value must be [N, H, D] tensors of one shape and type")
+        if tuple(key.shape[1:]) != (self.heads, self.head_dim):
+            raise ValueError(f"rows must be [N, {self.heads}, {self.head_dim}]")
+        if key.device != self.device or value.device != self.device:
+            raise ValueError(f"rows must lie on {self.device}")
+        _check("slots", slots, torch.int64, (key.shape[0],), self.device)
+        _check("seqs", seqs, torch.int32, (key.shape[0],), self.device)
+        raise ValueError("key, value, slots and seqs do not belong to this cache")
 
     def attend(self, query: torch.Tensor, current_key: torch.Tensor | None = None,
                current_value: torch.Tensor | None = None, *, scaling: float | None = None, causal: bool = True,
@@ -265,10 +291,11 @@ class _Call:
     """What one form of an in-place attention call (its tensors' shapes, strides and types)
     passes besides the pointers."""
 
-    __slots__ = ("heads", "geometry", "sq", "tc", "sk", "sv", "shape", "so", "scale", "causal", "nbytes")
+    __slots__ = ("run", "device", "heads", "geometry", "sq", "tc", "sk", "sv", "shape", "so", "scale", "causal", "nbytes", "packed")
 
 
 _MAX_FORMS = 256     # remembered forms per cache; a loop has a few
+_NO_BLOCK = MaBlock()
 
 
 def _attend(query, source, desc, current_key, current_value, scaling, causal, out, workspace):
@@ -278,12 +305,12 @@ def _attend(query, source, desc, current_key, current_value, scaling, causal, ou
     forms = form = call = None
     if isinstance(source, PagedCache):
         forms = source._forms
-        form = (query.shape, query.stride(), query.dtype, query.device, scaling, causal,
+        form = (query.shape, query.stride(), query.dtype, query.get_device(), scaling, causal,
                 None if current_key is None else (current_key.shape, current_key.stride(), current_key.dtype,
-                                                  current_key.device),
+                                                  current_key.get_device()),
                 None if current_value is None else (current_value.shape, current_value.stride(), current_value.dtype,
-                                                    current_value.device),
-                None if out is None else (out.shape, out.stride(), out.dtype, out.device))
+                                                    current_value.get_device()),
+                None if out is None else (out.shape, out.stride(), out.dtype, out.get_device()))
         call = forms.get(form)
     if call is None:
         if query.dtype == torch.bfloat16 and current_value is not None and current_key is not None:
@@ -312,11 +339,12 @@ def _attend(query, source, desc, current_key, current_value, scaling, causal, ou
         raise ValueError("out must start on a 16-byte boundary")
     if desc is None:
         desc = kv_descriptor(source, batch=query.shape[0], heads=call.heads, head_dim=query.shape[3])
-    o = torch.empty(call.shape, device=query.device, dtype=query.dtype) if out is None else out
-    ws = _workspace(query.device, "decode", call.nbytes, workspace)
-    rc = _lib.lib().ma_decode_attention(
-        MaRows(q, _lib.MA_BF16, *call.geometry, call.sq), desc.kv, call.heads, MaBlock(k, v, call.tc, call.sk, call.sv),
-        call.scale, call.causal, o.data_ptr(), call.so, ws.data_ptr(), ws.numel(), _lib.stream_handle(query.device))
+    o = out if out is not None else torch.empty_like(query) if call.packed else query.new_empty(call.shape)
+    dev = call.device
+    ws, nbytes = _scratch(dev, "decode", call.nbytes, workspace)
+    rc = call.run(MaRows(q, _lib.MA_BF16, *call.geometry, call.sq), desc.kv, call.heads,
+                  MaBlock(k, v, call.tc, call.sk, call.sv) if call.tc else _NO_BLOCK,
+                  call.scale, call.causal, o.data_ptr(), call.so, ws, nbytes, _lib.stream_handle(dev))
     if rc == _lib.MA_ERR_UNSUPPORTED:
         return _attend_general(query, source, current_key, current_value, scaling, causal, out)
     if rc:
@@ -360,10 +388,11 @@ def _attend_form(query, source, current_key, current_value, scaling, causal, out
             cached or (source.nq > 0 and source.nf == 0 and source.kmode == 1)):
         return None
     call = _Call()
+    call.run, call.device = _lib.lib().ma_decode_attention, query.device
     call.heads, call.geometry, call.tc = heads, (b, hq, t, d), tc
     call.sq = i64(*query.stride()[:3])
     call.sk, call.sv = (i64(*current_key.stride()[:3]), i64(*current_value.stride()[:3])) if tc else (i64(0, 0, 0), i64(0, 0, 0))
-    call.shape = (b, hq, t, d)
+    call.shape, call.packed = (b, hq, t, d), query.is_contiguous()
     call.so = i64(hq * t * d, t * d, d) if out is None else i64(*out.stride()[:3])
     call.scale = d ** -0.5 if scaling is None else float(scaling)
     call.causal = 1 if causal else 0
@@ -405,7 +434,38 @@ def verify_drafts(target: torch.Tensor, draft: torch.Tensor | None, tokens: torc
     Returns (accepted [B] int32, tokens [B, K + 1] int32: the accepted drafts, the next token,
     then -1); tokens[b, accepted[b]] is -1 only when p_a has no mass.
     """
-    if target.ndim != 3 or target.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+    shape, index = target.shape, target.get_device()
+    b, k1, v = shape if len(shape) == 3 else (0, 0, 0)
+    k = k1 - 1
+    code = _PROBABILITIES.get(target.dtype)
+    if (code is None or index < 0 or b < 1 or k < 0 or v < 1 or tokens.dtype is not torch.int32
+            or tokens.shape != (b, k) or tokens.get_device() != index or not tokens.is_contiguous()
+            or uniforms.dtype is not torch.float32 or uniforms.shape != (b, k1) or uniforms.get_device() != index
+            or not uniforms.is_contiguous() or (target.stride(2) != 1 and v > 1)
+            or (counts is not None and (counts.dtype is not torch.int32 or counts.shape != (b,)
+                                        or counts.get_device() != index or not counts.is_contiguous()))
+            or (draft is not None and (draft.dtype is not target.dtype or draft.shape != (b, k, v)
+                                       or draft.get_device() != index or (draft.stride(2) != 1 and v > 1)))):
+        _refuse_verify(target, draft, tokens, counts, uniforms)
+    dev = target.device
+    accepted = uniforms.new_empty(b, dtype=torch.int32) if counts is None else torch.empty_like(counts)
+    out = tokens.new_empty((b, k1))
+    ws, nbytes = _scratch(dev, "verify", verify_workspace_bytes(b, v), workspace)
+    rc = _lib.lib().ma_verify_drafts(
+        target.data_ptr(), None if draft is None else draft.data_ptr(), code, b, k, v, _strides(target.stride()[:2]),
+        None if draft is None else _strides(draft.stride()[:2]), tokens.data_ptr(),
+        None if counts is None else counts.data_ptr(), uniforms.data_ptr(), accepted.data_ptr(), out.data_ptr(), ws,
+        nbytes, _lib.stream_handle(dev))
+    if rc:
+        _lib.check("ma_verify_drafts", rc)
+    return accepted, out
+
+
+_PROBABILITIES = {torch.float32: _lib.MA_F32, torch.bfloat16: _lib.MA_BF16, torch.float16: _lib.MA_F16}
+
+
+def _refuse_verify(target, draft, tokens, counts, uniforms) -> None:
+    if target.ndim != 3 or target.dtype not in _PROBABILITIES:
         raise ValueError("target must be a float32, bfloat16 or float16 tensor [B, K + 1, V]")
     b, k1, v = target.shape
     k, dev = k1 - 1, target.device
@@ -415,22 +475,11 @@ def verify_drafts(target: torch.Tensor, draft: torch.Tensor | None, tokens: torc
         raise ValueError("target must be [B, K + 1, V] with B, V >= 1 and K >= 0")
     if target.stride(2) != 1 and v > 1:
         raise ValueError("target must have a contiguous vocabulary axis")
-    if draft is not None and (draft.dtype != target.dtype or draft.shape != (b, k, v) or draft.device != dev
+    if draft is not None and (draft.dtype != target.dtype or tuple(draft.shape) != (b, k, v) or draft.device != dev
                               or (draft.stride(2) != 1 and v > 1)):
         raise ValueError(f"draft must be a {target.dtype} tensor {(b, k, v)} on {dev} with a contiguous vocabulary axis")
     _check("tokens", tokens, torch.int32, (b, k), dev)
     _check("uniforms", uniforms, torch.float32, (b, k1), dev)
     if counts is not None:
         _check("counts", counts, torch.int32, (b,), dev)
-    lib = _lib.lib()
-    accepted = torch.empty(b, device=dev, dtype=torch.int32)
-    out = torch.empty((b, k1), device=dev, dtype=torch.int32)
-    ws = _workspace(dev, "verify", verify_workspace_bytes(b, v), workspace)
-    code = _lib.MA_F16 if target.dtype == torch.float16 else _lib.dtype_code(target.dtype)
-    rc = lib.ma_verify_drafts(target.data_ptr(), _lib.ptr(draft), code, b, k, v, _strides(target.stride()[:2]),
-                              _strides(draft.stride()[:2]) if draft is not None else None,
-                              tokens.data_ptr(), _lib.ptr(counts), uniforms.data_ptr(), accepted.data_ptr(),
-                              out.data_ptr(), ws.data_ptr(), ws.numel(), _lib.stream_handle(dev))
-    if rc:
-        _lib.check("ma_verify_drafts", rc)
-    return accepted, out
+    raise ValueError("the tensors do not belong together")
