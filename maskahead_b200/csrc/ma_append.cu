@@ -3,9 +3,9 @@
 //
 // Each row's 32-channel groups are quantized to the bytes that ma_quantize_tokens gives, so a
 // cache filled by prompts in one call and by single tokens in many holds the same. A thread has
-// 8 channels: a group's minimum and maximum meet in two shuffles, its 16 payload bytes are
-// four neighbouring words, and a row of 128 channels is read and written by 16 neighbouring
-// threads. A block takes a run of consecutive tokens, so that a thread keeps its head, its
+// 16 channels, half a group, so that what a row costs beside its elements (its slot, the group's
+// minimum and maximum, its step) is shared by many; a row of 128 channels is read and written by
+// 8 neighbouring threads. A block takes a run of consecutive tokens, so that a thread keeps its head, its
 // channels and, until the request changes, its divisors and their reciprocals.
 //
 // Bound: HBM (bf16 D = 128: 256 B in, 80 B to the pool, 256 B of values out per row) with the
@@ -24,36 +24,39 @@ namespace ma {
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 constexpr int kGroup = 32;
+constexpr int kEach = 16;              // channels per thread
+constexpr int kPeers = kGroup / kEach; // threads per group
 
-// ---- one group's 8 channels of a thread: x (keys already divided) -> codes, step and minimum
+// ---- a thread's channels of one group: x (keys already divided) -> codes, step and minimum
 struct Quantized {
-  uint32_t packed;
+  uint32_t packed[kEach / 8];
   __half step, low;
-  float code[8];
+  float code[kEach];
 };
 
 // 32-bit rows: the quantizer's operations as they are.
-__device__ __forceinline__ Quantized quantize(const float x[8]) {
+__device__ __forceinline__ Quantized quantize(const float x[kEach]) {
   float mn = x[0], mx = x[0];
 #pragma unroll
-  for (int e = 1; e < 8; ++e) {
+  for (int e = 1; e < kEach; ++e) {
     mn = fminf(mn, x[e]);
     mx = fmaxf(mx, x[e]);
   }
 #pragma unroll
-  for (int o = 1; o < kGroup / 8; o <<= 1) {
+  for (int o = 1; o < kPeers; o <<= 1) {
     mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   }
   const float s = fmaxf((mx - mn) / 15.0f, 1e-8f);
   Quantized r;
-  r.packed = 0u;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
+  for (int w = 0; w < kEach / 8; ++w) r.packed[w] = 0u;
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
     r.code[e] = fminf(fmaxf(rintf((x[e] - mn) / s), 0.f), 15.f);
-    r.packed |= (uint32_t)r.code[e] << (4 * e);
+    r.packed[e / 8] |= (uint32_t)r.code[e] << (4 * (e & 7));
   }
   r.step = __float2half_rn(s);
   r.low = __float2half_rn(mn);
@@ -66,11 +69,15 @@ __device__ __forceinline__ float lo_float(uint32_t x) { return __uint_as_float(x
 __device__ __forceinline__ float hi_float(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
 
 // bf16 rows, x in pairs: every operation rounded to bf16, as the quantizer does it.
-__device__ __forceinline__ Quantized quantize(const uint32_t x[4]) {
-  __nv_bfloat162 mn = __hmin2(__hmin2(pair(x[0]), pair(x[1])), __hmin2(pair(x[2]), pair(x[3])));
-  __nv_bfloat162 mx = __hmax2(__hmax2(pair(x[0]), pair(x[1])), __hmax2(pair(x[2]), pair(x[3])));
+__device__ __forceinline__ Quantized quantize(const uint32_t x[kEach / 2]) {
+  __nv_bfloat162 mn = pair(x[0]), mx = pair(x[0]);
 #pragma unroll
-  for (int o = 1; o < kGroup / 8; o <<= 1) {
+  for (int e = 1; e < kEach / 2; ++e) {
+    mn = __hmin2(mn, pair(x[e]));
+    mx = __hmax2(mx, pair(x[e]));
+  }
+#pragma unroll
+  for (int o = 1; o < kPeers; o <<= 1) {
     mn = __hmin2(mn, pair(__shfl_xor_sync(0xffffffffu, bits(mn), o)));
     mx = __hmax2(mx, pair(__shfl_xor_sync(0xffffffffu, bits(mx), o)));
   }
@@ -81,11 +88,11 @@ __device__ __forceinline__ Quantized quantize(const uint32_t x[4]) {
   const float rs = __fdividef(1.0f, s);
   const __nv_bfloat162 low2 = __float2bfloat162_rn(low);
   Quantized r;
-  uint32_t c[4];
+  uint32_t c[kEach / 2];
   // non-finite rows and steps (s or its reciprocal out of range): the operations as they are
   const bool plain = d < 1e30f;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
+  for (int e = 0; e < kEach / 2; ++e) {
     const uint32_t a = bits(__hsub2(pair(x[e]), low2));
     __nv_bfloat162 t;               // in [0, 15.1] or NaN (-> 0)
     if (plain) {
@@ -95,14 +102,18 @@ __device__ __forceinline__ Quantized quantize(const uint32_t x[4]) {
       t = __hmin2(t, __float2bfloat162_rn(15.f));
     }
     // 128 + t rounds t to the nearest whole number, ties to even, and leaves it in the low bits
-    c[e] = bits(__hadd2(t, __float2bfloat162_rn(128.f)));
-    r.code[2 * e] = lo_float(c[e]) - 128.f;
-    r.code[2 * e + 1] = hi_float(c[e]) - 128.f;
-    c[e] &= 0x000f000fu;
+    const __nv_bfloat162 w = __hadd2(t, __float2bfloat162_rn(128.f));
+    const uint32_t code = bits(__hsub2(w, __float2bfloat162_rn(128.f)));
+    r.code[2 * e] = lo_float(code);
+    r.code[2 * e + 1] = hi_float(code);
+    c[e] = bits(w) & 0x000f000fu;
   }
-  // (c0, c1), (c2, c3) in 16-bit halves -> four nibbles of a half word
-  const uint32_t u = c[0] + c[1] * 256u, v = c[2] + c[3] * 256u;
-  r.packed = __byte_perm(u | u >> 12, v | v >> 12, 0x5410);
+#pragma unroll
+  for (int w = 0; w < kEach / 8; ++w) {
+    // (c0, c1), (c2, c3) in 16-bit halves -> four nibbles of a half word
+    const uint32_t u = c[4 * w] + c[4 * w + 1] * 256u, v = c[4 * w + 2] + c[4 * w + 3] * 256u;
+    r.packed[w] = __byte_perm(u | u >> 12, v | v >> 12, 0x5410);
+  }
   r.step = __float2half_rn(s);
   r.low = __float2half_rn(low);
   return r;
@@ -111,12 +122,12 @@ __device__ __forceinline__ Quantized quantize(const uint32_t x[4]) {
 // A thread's divisors, and for bf16 rows their reciprocals, a little too large and too small.
 template <bool BF16>
 struct Divisors {
-  float kc[8], above[BF16 ? 8 : 1], below[BF16 ? 8 : 1];
+  float kc[kEach], above[BF16 ? kEach : 1], below[BF16 ? kEach : 1];
   bool usable;
   __device__ __forceinline__ void load(const float* p) {
     usable = true;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+    for (int e = 0; e < kEach; ++e) {
       kc[e] = p[e];
       if (BF16) {
         const float r = 1.0f / kc[e];
@@ -128,50 +139,61 @@ struct Divisors {
   }
 };
 
-__device__ __forceinline__ void divide(const Divisors<false>& k, float x[8]) {
+__device__ __forceinline__ void divide(const Divisors<false>& k, float x[kEach]) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] /= k.kc[e];
+  for (int e = 0; e < kEach; ++e) x[e] /= k.kc[e];
 }
-__device__ __forceinline__ void divide(const Divisors<true>& k, uint32_t x[4]) {
-  uint32_t y[4], apart = k.usable ? 0u : 1u;
+__device__ __forceinline__ void divide(const Divisors<true>& k, uint32_t x[kEach / 2]) {
+  uint32_t y[kEach / 2], apart = k.usable ? 0u : 1u;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
+  for (int e = 0; e < kEach / 2; ++e) {
     const float a = lo_float(x[e]), b = hi_float(x[e]);
     y[e] = bits(__floats2bfloat162_rn(a * k.above[2 * e], b * k.above[2 * e + 1]));
     apart |= y[e] ^ bits(__floats2bfloat162_rn(a * k.below[2 * e], b * k.below[2 * e + 1]));
   }
   if (apart) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = bits(__floats2bfloat162_rn(lo_float(x[e]) / k.kc[2 * e], hi_float(x[e]) / k.kc[2 * e + 1]));
+    for (int e = 0; e < kEach / 2; ++e)
+      y[e] = bits(__floats2bfloat162_rn(lo_float(x[e]) / k.kc[2 * e], hi_float(x[e]) / k.kc[2 * e + 1]));
   }
 #pragma unroll
-  for (int e = 0; e < 4; ++e) x[e] = y[e];
+  for (int e = 0; e < kEach / 2; ++e) x[e] = y[e];
 }
 
-__device__ __forceinline__ void load_row(const float* p, float x[8]) { load8(p, x); }
-__device__ __forceinline__ void load_row(const __nv_bfloat16* p, uint32_t x[4]) {
-  const uint4 u = *reinterpret_cast<const uint4*>(p);
-  x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
+__device__ __forceinline__ void load_row(const float* p, float x[kEach]) {
+#pragma unroll
+  for (int e = 0; e < kEach; e += 4) {
+    const float4 u = *reinterpret_cast<const float4*>(p + e);
+    x[e] = u.x; x[e + 1] = u.y; x[e + 2] = u.z; x[e + 3] = u.w;
+  }
 }
-__device__ __forceinline__ void store_row(float* p, const float f[8]) {
-  reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
-  reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+__device__ __forceinline__ void load_row(const __nv_bfloat16* p, uint32_t x[kEach / 2]) {
+#pragma unroll
+  for (int e = 0; e < kEach / 2; e += 4) {
+    const uint4 u = *reinterpret_cast<const uint4*>(p + 2 * e);
+    x[e] = u.x; x[e + 1] = u.y; x[e + 2] = u.z; x[e + 3] = u.w;
+  }
 }
-__device__ __forceinline__ void store_row(__nv_bfloat16* p, const float f[8]) {
-  *reinterpret_cast<uint4*>(p) = float8_to_bf16x8(f);
+__device__ __forceinline__ void store_row(float* p, const float f[kEach]) {
+#pragma unroll
+  for (int e = 0; e < kEach; e += 4) *reinterpret_cast<float4*>(p + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+}
+__device__ __forceinline__ void store_row(__nv_bfloat16* p, const float f[kEach]) {
+#pragma unroll
+  for (int e = 0; e < kEach; e += 8) *reinterpret_cast<uint4*>(p + e) = float8_to_bf16x8(f + e);
 }
 
 template <typename T, int D, bool KEY>
 __device__ __forceinline__ void append_run(const AppendParams& p, int first, int last, int step, int h, int c) {
   using Raw = typename std::conditional<sizeof(T) == 2, uint32_t, float>::type;
-  constexpr int kRaw = sizeof(T) == 2 ? 4 : 8;
-  const T* src = reinterpret_cast<const T*>(KEY ? p.k : p.v) + (int64_t)h * (KEY ? p.sk[1] : p.sv[1]) + c * 8;
+  constexpr int kRaw = sizeof(T) == 2 ? kEach / 2 : kEach;
+  const T* src = reinterpret_cast<const T*>(KEY ? p.k : p.v) + (int64_t)h * (KEY ? p.sk[1] : p.sv[1]) + c * kEach;
   const int64_t stride = KEY ? p.sk[0] : p.sv[0];
   T* rows = reinterpret_cast<T*>(KEY ? p.k_rows : p.v_rows);
   const int64_t* sq = KEY ? p.kv.skq : p.kv.svq;
   const int64_t* sc = KEY ? p.kv.sks : p.kv.svs;
-  uint8_t* pay = const_cast<uint8_t*>(KEY ? p.kv.kq : p.kv.vq) + (int64_t)h * sq[1] + c * 4;
-  const int64_t sc0 = (int64_t)h * sc[1] + c / 4;
+  uint8_t* pay = const_cast<uint8_t*>(KEY ? p.kv.kq : p.kv.vq) + (int64_t)h * sq[1] + c * (kEach / 2);
+  const int64_t sc0 = (int64_t)h * sc[1] + c / kPeers;
   __half* scale = reinterpret_cast<__half*>(const_cast<uint16_t*>(KEY ? p.kv.ks : p.kv.vs)) + sc0;
   __half* zero = reinterpret_cast<__half*>(const_cast<uint16_t*>(KEY ? p.kv.kz : p.kv.vz)) + sc0;
   const int64_t limit = (int64_t)p.kv.num_pages * p.kv.page_size;
@@ -202,7 +224,7 @@ __device__ __forceinline__ void append_run(const AppendParams& p, int first, int
     if (KEY) {
       const int want = owned ? seq : 0;
       if (want != held) {
-        kd.load(p.kv.kchan + (int64_t)want * p.kv.skc[0] + (int64_t)h * p.kv.skc[1] + c * 8);
+        kd.load(p.kv.kchan + (int64_t)want * p.kv.skc[0] + (int64_t)h * p.kv.skc[1] + c * kEach);
         held = want;
       }
       divide(kd, x);
@@ -211,16 +233,19 @@ __device__ __forceinline__ void append_run(const AppendParams& p, int first, int
     if (!valid) continue;
     if (rows != nullptr) {
       const float s = __half2float(q.step), z = __half2float(q.low);
-      float back[8];
+      float back[kEach];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
+      for (int e = 0; e < kEach; ++e) {
         back[e] = fmaf(q.code[e], s, z);
         if (KEY) back[e] *= kd.kc[e];
-        if (!owned) back[e] = 0.f;
       }
-      store_row(rows + ((int64_t)i * p.H + h) * D + c * 8, back);
+      if (!owned) {
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) back[e] = 0.f;
+      }
+      store_row(rows + ((int64_t)i * p.H + h) * D + c * kEach, back);
     }
-    if (!owned || slot < 0 || slot >= limit) continue;
+    if (!owned || (uint64_t)slot >= (uint64_t)limit) continue;
     int64_t page, at;
     if (slot <= 0x7fffffffLL) {
       page = p.page_div.div((int)slot);
@@ -229,8 +254,8 @@ __device__ __forceinline__ void append_run(const AppendParams& p, int first, int
       page = slot / p.kv.page_size;
       at = slot - page * p.kv.page_size;
     }
-    *reinterpret_cast<uint32_t*>(pay + page * sq[0] + at * sq[2]) = q.packed;
-    if ((c & 3) == 0) {
+    *reinterpret_cast<uint2*>(pay + page * sq[0] + at * sq[2]) = make_uint2(q.packed[0], q.packed[1]);
+    if (c % kPeers == 0) {
       const int64_t o = page * sc[0] + at * sc[2];
       scale[o] = q.step;
       zero[o] = q.low;
@@ -241,7 +266,7 @@ __device__ __forceinline__ void append_run(const AppendParams& p, int first, int
 // grid: (runs of tokens, heads / heads per block, K or V)
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant__ AppendParams p) {
-  constexpr int kLanes = D / 8;                    // threads per row
+  constexpr int kLanes = D / kEach;                // threads per row
   const int c = threadIdx.x % kLanes, row = threadIdx.x / kLanes;
   const int sub = row / p.heads_per_block, h = blockIdx.y * p.heads_per_block + row - sub * p.heads_per_block;
   const int step = kThreads / kLanes / p.heads_per_block;
@@ -254,12 +279,12 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
 
 template <typename T, int D>
 int launch(AppendParams& p, cudaStream_t st) {
-  constexpr int kRows = kThreads / (D / 8);
+  constexpr int kRows = kThreads / (D / kEach);
   p.heads_per_block = kRows % p.H == 0 ? p.H : 1;
   const int step = kRows / p.heads_per_block, groups = p.H / p.heads_per_block;
-  // runs of at least one round of the block; at most about 8 blocks an SM over K, V and the heads
+  // runs of at least one round of the block; at most about 16 blocks an SM over K, V and the heads
   int64_t runs = ((int64_t)p.N + step - 1) / step;
-  const int64_t cap = ((int64_t)device_sm_count() * 8 + 2 * groups - 1) / (2 * groups);
+  const int64_t cap = ((int64_t)device_sm_count() * 16 + 2 * groups - 1) / (2 * groups);
   if (runs > cap) runs = cap;
   const int64_t per = ((int64_t)p.N + runs - 1) / runs;
   p.run = (int)((per + step - 1) / step * step);

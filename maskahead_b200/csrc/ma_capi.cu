@@ -912,8 +912,10 @@ int ma_append_tokens(const ma_kv* pool, int B, int H, int D, const void* k, cons
 
 size_t ma_verify_drafts_workspace(int B, int V) {
   if (B <= 0 || V <= 0) return 0;
-  int span, spans;
-  plan_verify(B, V, span, spans);
+  VerifyPlan wide, narrow;      // 32- and 16-bit rows
+  plan_verify(B, V, 4, wide);
+  plan_verify(B, V, 2, narrow);
+  const size_t spans = wide.spans > narrow.spans ? wide.spans : narrow.spans;
   return 512 + kVerifyTickets * sizeof(unsigned) + (size_t)B * spans * sizeof(unsigned long long);
 }
 
@@ -942,7 +944,12 @@ int ma_verify_drafts(const void* target, const void* draft, int32_t dtype, int B
   p.B = B;
   p.K = K;
   p.V = V;
-  plan_verify(B, V, p.span, p.spans);
+  VerifyPlan plan;
+  plan_verify(B, V, dtype == MA_F32 ? 4 : 2, plan);
+  p.ctas = plan.ctas;
+  p.share = plan.share;
+  p.per_warp = plan.per_warp;
+  p.spans = plan.spans;
   p.accepted = accepted;
   p.out = out;
   char* base = align256(workspace) + 256;

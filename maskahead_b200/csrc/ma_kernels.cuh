@@ -265,12 +265,16 @@ struct VerifyParams {
   int64_t st[2], sd[2];         // strides over (request, position)
   const int32_t *tokens, *counts;
   const float* uniforms;        // [B, K + 1]
-  int B, K, V, span, spans;
+  int B, K, V;
+  int ctas, share, per_warp, spans;   // VerifyPlan
   int32_t *accepted, *out;      // [B], [B, K + 1]
   unsigned* tickets;            // [B], zero between calls
   unsigned long long* sums;     // [B][spans]
 };
-void plan_verify(int B, int V, int& span, int& spans);
+struct VerifyPlan {
+  int ctas, share, per_warp, spans;   // CTAs per request, elements and spans per warp, spans per request
+};
+void plan_verify(int B, int V, int elem, VerifyPlan& plan);
 int verify_max_requests();
 int launch_verify_drafts(const VerifyParams& p, int dtype, cudaStream_t st);
 

@@ -8,10 +8,12 @@
 // numbers do not depend on their order, so the token does not depend on the split.
 //
 // Bound: HBM, one row of p and one of q per request (the other rows are read at one element
-// each). A warp sums one span of one request's row; the last CTA of the request to arrive
-// finds the span that holds the threshold and rescans that span alone, from L2. The spans make
-// about one wave of CTAs, because every CTA first finds the accepted run for itself (two
-// dependent loads, 1.5 us).
+// each). A warp sums its share of a request's row in spans of 2 KB, which cp.async brings into its
+// own ring of shared memory by 16-byte pieces -- rows of an odd vocabulary in 16 bits lie on any
+// even address, and element loads kept too few bytes in flight (800 rows of 100003: 116 us
+// against 58). The last CTA of the request to arrive finds the span that holds the threshold and rescans
+// that span alone, from L2. Each CTA first finds the accepted run for itself (two dependent loads,
+// 1.5 us).
 //
 // floor(r 2^40) takes no conversion (those run at an eighth of the FMA rate): with t = r 2^20 +
 // 2^23 truncated, t's low bits are the upper 20 bits of the weight, and the remainder gives the
@@ -22,16 +24,21 @@ namespace ma {
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
-constexpr int kMaxSpans = 1024;
-constexpr int kMaxSpan = 4096;          // elements: what the last CTA rescans
+constexpr int kMaxSpans = 2048;
+constexpr int kSpanBytes = 2048;        // of a span of p or q: what a warp copies at once, and the last CTA rescans
+constexpr int kStages = 2;
+constexpr int kBuffer = kSpanBytes + 16;                        // a span from the 16-byte boundary at or before it
+constexpr int kRingBytes = kWarps * kStages * 2 * kBuffer;
 constexpr int kMaxRequests = 65535;
 constexpr uint32_t kMagicBits = 0x4B000000u;       // 2^23
 
-__device__ __forceinline__ float value(const float* p, int64_t i) { return __ldg(p + i); }
-__device__ __forceinline__ float value(const __nv_bfloat16* p, int64_t i) { return __bfloat162float(p[i]); }
-__device__ __forceinline__ float value(const __half* p, int64_t i) { return __half2float(p[i]); }
+__device__ __forceinline__ float value_of(float x) { return x; }
+__device__ __forceinline__ float value_of(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float value_of(__half x) { return __half2float(x); }
+template <typename T>
+__device__ __forceinline__ float value(const T* p, int64_t i) { return value_of(p[i]); }
 
 // The halves of floor(r 2^40), r in [0, 1], each plus the bits of 2^23.
 __device__ __forceinline__ void weight_halves(float r, uint32_t& hi, uint32_t& lo) {
@@ -87,71 +94,108 @@ struct Row {
     weight_halves(rest(v), hi, lo);
     return v == dropped ? 0ull : join(hi, lo, 1);
   }
-  // the sum over [begin, end) by one warp: at most kMaxSpan elements, 128 a lane
-  template <bool Q>
-  __device__ __forceinline__ unsigned long long span(int begin, int end) const {
-    const int lane = threadIdx.x & 31;
+};
+
+// Elements [begin, end) of a row to shared memory, by one warp, from the 16-byte boundary at or
+// before the first; returns how many bytes that is before it. (The bytes before a row are of its
+// tensor's storage; nothing past `end` is read.)
+template <typename T>
+__device__ __forceinline__ void copy_span(uint32_t dst, const T* row, int begin, int end) {
+  const uintptr_t first = reinterpret_cast<uintptr_t>(row + begin), last = reinterpret_cast<uintptr_t>(row + end);
+  uintptr_t at = (first & ~uintptr_t(15)) + (threadIdx.x & 31) * 16;
+#pragma unroll
+  for (int e = 0; e < (kBuffer + 511) / 512; ++e, at += 512) {
+    if (at < last) {
+      const uint32_t bytes = (uint32_t)(last - at < 16 ? last - at : 16);
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n"
+                   ::"r"(dst + (uint32_t)(at - (first & ~uintptr_t(15)))), "l"(reinterpret_cast<const void*>(at)), "r"(bytes) : "memory");
+    }
+  }
+}
+template <typename T>
+__device__ __forceinline__ const T* span_at(const char* buffer, const T* row, int begin) {
+  return reinterpret_cast<const T*>(buffer + (reinterpret_cast<uintptr_t>(row + begin) & 15));
+}
+
+// The sums of the spans of [begin, end) by one warp, to sums[0 .. count).
+template <typename T, bool Q>
+__device__ __forceinline__ void sum_spans(const Row<T>& row, int begin, int end, int count, char* ring,
+                                          unsigned long long* sums) {
+  constexpr int kSpan = kSpanBytes / sizeof(T);
+  const int lane = threadIdx.x & 31;
+  const uint32_t base = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
+  auto issue = [&](int j) {
+    const int first = begin + j * kSpan, last = min(end, first + kSpan);
+    if (j < count && first < last) {
+      copy_span(base + (j % kStages) * 2 * kBuffer, row.p, first, last);
+      if (Q) copy_span(base + ((j % kStages) * 2 + 1) * kBuffer, row.q, first, last);
+    }
+    asm volatile("cp.async.commit_group;\n" ::: "memory");
+  };
+#pragma unroll
+  for (int j = 0; j < kStages - 1; ++j) issue(j);
+  for (int j = 0; j < count; ++j) {
+    issue(j + kStages - 1);
+    asm volatile("cp.async.wait_group %0;\n" ::"n"(kStages - 1) : "memory");
+    __syncwarp();
+    const int first = begin + j * kSpan, last = min(end, first + kSpan);
+    const T* a = span_at(ring + (j % kStages) * 2 * kBuffer, row.p, first) + lane;
+    const T* b = Q ? span_at(ring + ((j % kStages) * 2 + 1) * kBuffer, row.q, first) + lane : nullptr;
     uint32_t hi = 0u, lo = 0u, n = 0u;
-    int v = begin + lane;
-    for (; v + 7 * 32 < end; v += 8 * 32, n += 8) {
-      float a[8], b[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        a[e] = value(p, v + e * 32);
-        b[e] = Q ? value(q, v + e * 32) : 0.f;
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
+    if (last - first == kSpan) {
+#pragma unroll 8
+      for (int e = 0; e < kSpan / 32; ++e) {
         uint32_t x, y;
-        weight_halves(__saturatef(a[e] - b[e]), x, y);
+        weight_halves(__saturatef(Q ? value_of(a[e * 32]) - value_of(b[e * 32]) : value_of(a[e * 32])), x, y);
+        hi += x;
+        lo += y;
+      }
+      n = kSpan / 32;
+    } else {
+      for (int v = first + lane; v < last; v += 32, a += 32, ++n) {
+        uint32_t x, y;
+        weight_halves(__saturatef(Q ? value_of(*a) - value_of(b[n * 32]) : value_of(*a)), x, y);
         hi += x;
         lo += y;
       }
     }
-    for (; v < end; v += 32, ++n) {
-      uint32_t x, y;
-      weight_halves(rest(v), x, y);
-      hi += x;
-      lo += y;
-    }
     unsigned long long s = join(hi, lo, n);
-    if (dropped >= begin && dropped < end && ((dropped - begin) & 31) == lane) {      // the lane that counted it
+    if (row.dropped >= first && row.dropped < last && ((row.dropped - first) & 31) == lane) {      // the lane that counted it
       uint32_t x, y;
-      weight_halves(rest(dropped), x, y);
+      weight_halves(row.rest(row.dropped), x, y);
       s -= join(x, y, 1);
     }
-    return warp_sum64(s);
+    s = warp_sum64(s);
+    if (lane == 0) __stcg(&sums[j], s);
+    __syncwarp();                  // the span is read before its place is filled again
   }
-  __device__ __forceinline__ unsigned long long span(int begin, int end) const {
-    return q != nullptr ? span<true>(begin, end) : span<false>(begin, end);
-  }
-};
+}
 
 // The first element of [begin, end) whose inclusive sum (from `before`) is above the mark, by the
-// whole CTA, kMaxSpan elements at a time; -1 when there is none.
+// whole CTA, kScan elements at a time; -1 when there is none.
 template <typename T>
 __device__ int find_crossing(const Row<T>& row, int begin, int end, unsigned long long before, unsigned long long mark,
                              unsigned long long* sWarp, int* sFound) {
-  constexpr int kEach = kMaxSpan / kThreads;
-  for (int v0 = begin; v0 < end; v0 += kMaxSpan) {
+  constexpr int kScan = 1024, kEach = kScan / kThreads;
+  for (int v0 = begin; v0 < end; v0 += kScan) {
     const int per = min(kEach, (end - v0 + kThreads - 1) / kThreads);       // consecutive elements of a thread
-    unsigned long long w[kEach], mine = 0, total;
-#pragma unroll
+    unsigned long long mine = 0, total;
+#pragma unroll 4
     for (int e = 0; e < kEach; ++e) {
       const int v = v0 + threadIdx.x * per + e;
-      w[e] = e < per && v < end ? row(v) : 0ull;
-      mine += w[e];
+      mine += e < per && v < end ? row(v) : 0ull;
     }
     const unsigned long long incl = before + block_scan(mine, total, sWarp);
     if (threadIdx.x == 0) *sFound = -1;
     __syncthreads();
-    if (incl > mark && incl - mine <= mark) {                // exactly one thread
+    if (incl > mark && incl - mine <= mark) {                // exactly one thread: its elements once more
       unsigned long long at = incl - mine;
-#pragma unroll
-      for (int e = 0; e < kEach; ++e) {
-        if (at <= mark && at + w[e] > mark) *sFound = v0 + threadIdx.x * per + e;
-        at += w[e];
+      int v = v0 + threadIdx.x * per;
+      for (;; ++v) {
+        at += row(v);
+        if (at > mark) break;
       }
+      *sFound = v;
     }
     __syncthreads();
     const int found = *sFound;
@@ -166,26 +210,38 @@ __device__ __forceinline__ unsigned long long mark_of(unsigned long long total, 
   return (total >> 24) * k + (((total & 0xffffffull) * k) >> 24);
 }
 
+// Span c of a row: a warp's share of `share` consecutive elements is per_warp spans. Those past the
+// row's end are empty.
+template <typename T>
+__device__ __forceinline__ void span_range(const VerifyParams& p, int c, int& begin, int& end) {
+  constexpr int kSpan = kSpanBytes / sizeof(T);
+  const int w = c / p.per_warp, j = c - w * p.per_warp;
+  const int64_t lo = (int64_t)w * p.share + j * kSpan;
+  begin = (int)min((int64_t)p.V, lo);
+  end = (int)min((int64_t)p.V, lo + kSpan);
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant__ VerifyParams p) {
+  extern __shared__ __align__(16) char sRing[];
   __shared__ unsigned long long sWarp[kWarps];
-  __shared__ int sRun, sLast, sFound, sSpan;
+  __shared__ int sRun, sCount, sLast, sFound, sSpan;
   __shared__ unsigned long long sBefore;
   const int b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const T* target = reinterpret_cast<const T*>(p.target) + (int64_t)b * p.st[0];
   const T* draft = p.draft == nullptr ? nullptr : reinterpret_cast<const T*>(p.draft) + (int64_t)b * p.sd[0];
-  const int n = min(max(p.counts == nullptr ? p.K : p.counts[b], 0), p.K);
   if (warp == 0) {       // the accepted run: the first refused draft, 32 at a time
+    const int n = min(max(p.counts == nullptr ? p.K : p.counts[b], 0), p.K);
     int run = n;
-    for (int i0 = 0; i0 < n; i0 += 32) {
+    for (int i0 = 0; i0 < p.K; i0 += 32) {      // (loads of unused drafts too: they do not wait for the count)
       const int i = i0 + lane;
-      bool good = true;
-      if (i < n) {
+      bool good = i >= n;
+      if (i < p.K) {
         const int x = p.tokens[(int64_t)b * p.K + i];
-        good = false;
+        const float u = p.uniforms[(int64_t)b * (p.K + 1) + i];
         if (x >= 0 && x < p.V) {
           const float q = draft == nullptr ? 1.f : value(draft, (int64_t)i * p.sd[1] + x);
-          good = p.uniforms[(int64_t)b * (p.K + 1) + i] * q < value(target, (int64_t)i * p.st[1] + x);
+          good |= u * q < value(target, (int64_t)i * p.st[1] + x);
         }
       }
       const unsigned bad = ~__ballot_sync(0xffffffffu, good);
@@ -194,21 +250,26 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant_
         break;
       }
     }
-    if (lane == 0) sRun = run;
+    if (lane == 0) {
+      sRun = run;
+      sCount = n;
+    }
   }
   __syncthreads();
-  const int run = sRun;
+  const int run = sRun, n = sCount;
   Row<T> row;
   row.p = target + (int64_t)run * p.st[1];
   row.q = run < n && draft != nullptr ? draft + (int64_t)run * p.sd[1] : nullptr;
   row.dropped = run < n && draft == nullptr ? p.tokens[(int64_t)b * p.K + run] : -1;
 
-  // ---- a span per warp
+  // ---- the spans, by warps
   unsigned long long* sums = p.sums + (int64_t)b * p.spans;
-  const int own = blockIdx.x * kWarps + warp;
-  if (own < p.spans) {
-    const unsigned long long sum = row.span(own * p.span, min(p.V, (own + 1) * p.span));
-    if (lane == 0) __stcg(&sums[own], sum);
+  {
+    const int w = blockIdx.x * kWarps + warp;
+    const int begin = (int)min((int64_t)p.V, (int64_t)w * p.share), end = (int)min((int64_t)p.V, (int64_t)(w + 1) * p.share);
+    char* ring = sRing + warp * kStages * 2 * kBuffer;
+    if (row.q != nullptr) sum_spans<T, true>(row, begin, end, p.per_warp, ring, sums + w * p.per_warp);
+    else sum_spans<T, false>(row, begin, end, p.per_warp, ring, sums + w * p.per_warp);
   }
   __threadfence();
   __syncthreads();
@@ -246,7 +307,9 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant_
       }
     }
     __syncthreads();
-    token = find_crossing(row, sSpan * p.span, min(p.V, (sSpan + 1) * p.span), sBefore, mark, sWarp, &sFound);
+    int begin, end;
+    span_range<T>(p, sSpan, begin, end);
+    token = find_crossing(row, begin, end, sBefore, mark, sWarp, &sFound);
   } else {
     // no residual mass (p <= q everywhere): the row of p itself, read again whole
     row.q = nullptr;
@@ -265,24 +328,46 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant_
 
 int verify_max_requests() { return kMaxRequests; }
 
-// Elements per span: about one wave of CTAs (5 an SM) over all requests, in steps of the 256
-// elements that a warp loads at once; at most kMaxSpans spans a row.
-void plan_verify(int B, int V, int& span, int& spans) {
-  const int64_t warps = (int64_t)device_sm_count() * 5 * kWarps;
-  int64_t n = ((int64_t)B * V + warps - 1) / warps;
-  n = (n + 255) / 256 * 256;
-  if (n > kMaxSpan) n = kMaxSpan;
-  while ((V + n - 1) / n > kMaxSpans) n += 256;
-  span = (int)n;
-  spans = (int)((V + n - 1) / n);
+// About 9 CTAs of 4 warps an SM, at least one a request: more than are resident at once (5),
+// because a refused draft doubles a request's bytes and later CTAs even that out. A warp's share
+// is whole spans.
+void plan_verify(int B, int V, int elem, VerifyPlan& plan) {
+  const int most = device_sm_count() * 9 / B > 1 ? device_sm_count() * 9 / B : 1;
+  const int span = kSpanBytes / elem;
+  const int64_t steps = ((int64_t)V + span - 1) / span;
+  for (int64_t each = (steps + (int64_t)most * kWarps - 1) / ((int64_t)most * kWarps);; ++each) {
+    const int64_t warps = (steps + each - 1) / each;
+    plan.ctas = (int)((warps + kWarps - 1) / kWarps);
+    plan.share = (int)(each * span);
+    plan.per_warp = (int)each;
+    plan.spans = plan.ctas * kWarps * plan.per_warp;
+    if (plan.spans <= kMaxSpans || each >= steps) break;
+  }
 }
 
-int launch_verify_drafts(const VerifyParams& p, int dtype, cudaStream_t st) {
-  const dim3 grid((p.spans + kWarps - 1) / kWarps, p.B);
-  if (dtype == MA_F32) verify_kernel<float><<<grid, kThreads, 0, st>>>(p);
-  else if (dtype == MA_BF16) verify_kernel<__nv_bfloat16><<<grid, kThreads, 0, st>>>(p);
-  else verify_kernel<__half><<<grid, kThreads, 0, st>>>(p);
+namespace {
+
+template <typename T>
+int launch(const VerifyParams& p, cudaStream_t st) {
+  static bool ready[64] = {false};       // per device: the attribute is set once
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return MA_ERR_CUDA;
+  if (dev < 0 || dev >= 64 || !ready[dev]) {
+    if (cudaFuncSetAttribute(verify_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes) != cudaSuccess ||
+        cudaFuncSetAttribute(verify_kernel<T>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) !=
+            cudaSuccess)
+      return MA_ERR_CUDA;
+    if (dev >= 0 && dev < 64) ready[dev] = true;
+  }
+  verify_kernel<T><<<dim3(p.ctas, p.B), kThreads, kRingBytes, st>>>(p);
   return cudaGetLastError() == cudaSuccess ? MA_OK : MA_ERR_CUDA;
+}
+
+}  // namespace
+
+int launch_verify_drafts(const VerifyParams& p, int dtype, cudaStream_t st) {
+  if (dtype == MA_F32) return launch<float>(p, st);
+  return dtype == MA_BF16 ? launch<__nv_bfloat16>(p, st) : launch<__half>(p, st);
 }
 
 }  // namespace ma
