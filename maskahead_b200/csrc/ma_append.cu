@@ -273,6 +273,8 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
   const int64_t begin = (int64_t)blockIdx.x * p.run;
   const int last = (int)min((int64_t)p.N, begin + p.run);
   const int first = (int)min((int64_t)last, begin + sub);
+  pdl_wait();
+  pdl_launch_dependents();
   if (blockIdx.z == 0) append_run<T, D, true>(p, first, last, step, h, c);
   else append_run<T, D, false>(p, first, last, step, h, c);
 }
@@ -290,8 +292,7 @@ int launch(AppendParams& p, cudaStream_t st) {
   p.run = (int)((per + step - 1) / step * step);
   runs = ((int64_t)p.N + p.run - 1) / p.run;
   p.page_div.set((uint32_t)p.kv.page_size);
-  append_kernel<T, D><<<dim3((unsigned)runs, groups, 2), kThreads, 0, st>>>(p);
-  return cudaGetLastError() == cudaSuccess ? MA_OK : MA_ERR_CUDA;
+  return launch_pdl(append_kernel<T, D>, dim3((unsigned)runs, groups, 2), dim3(kThreads), 0, st, p) == cudaSuccess ? MA_OK : MA_ERR_CUDA;
 }
 
 }  // namespace

@@ -501,6 +501,9 @@ __global__ void __launch_bounds__(W * 32, MINB) decode_attention_kernel(const __
   float2* sML = reinterpret_cast<float2*>(smem + NT * sizeof(QueryTile<D>));        // [1 + W][ROWS]
   float* sRows = reinterpret_cast<float*>(smem + NT * sizeof(QueryTile<D>) + (W + 1) * ROWS * 8);   // [1 + W][ROWS][kPad]
 
+  pdl_wait();
+  pdl_launch_dependents();
+
   // ---- this CTA's work. Whole shares: every sequence cut into shares of `per` units, one to a CTA,
   // when that takes few more units a CTA than equal ranges would (entering a sequence costs about
   // as much as kEnter units: its query rows, the first copies, its result); else equal ranges.
@@ -1027,8 +1030,7 @@ int launch(const DecodeParams& p, cudaStream_t st) {
       return MA_ERR_CUDA;
     if (dev >= 0 && dev < 64) ready[dev] = true;
   }
-  kernel<<<dim3(p.ctas, p.H * p.row_tiles), W * 32, smem, st>>>(p);
-  return cudaGetLastError() == cudaSuccess ? MA_OK : MA_ERR_CUDA;
+  return launch_pdl(kernel, dim3(p.ctas, p.H * p.row_tiles), dim3(W * 32), smem, st, p) == cudaSuccess ? MA_OK : MA_ERR_CUDA;
 }
 
 }  // namespace

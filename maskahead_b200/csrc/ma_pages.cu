@@ -84,6 +84,8 @@ __global__ void __launch_bounds__(kThreads) page_plan_kernel(const __grid_consta
   int* sWant = sLen + B;
   auto pages_of = [&](int len) { return len > 0 ? p.page_div.div(len - 1) + 1 : 0; };
 
+  pdl_wait();
+  pdl_launch_dependents();
   const int count = min(max(*p.free_count, 0), p.num_pages);
   const int64_t most = (int64_t)p.width * p.page_size;      // a length past its table is the table's
   const int longest = most < 0x7fffffffLL ? (int)most : 0x7fffffff;
@@ -285,8 +287,7 @@ int launch_page_plan(PagePlanParams& p, cudaStream_t st) {
   const int64_t cap = (int64_t)device_sm_count() * (p.B <= 1024 ? 2 : 1);
   p.page_div.set((uint32_t)p.page_size);
   grid = grid < 1 ? 1 : grid > cap ? cap : grid;
-  page_plan_kernel<<<(int)grid, kThreads, smem, st>>>(p);
-  return cudaGetLastError() == cudaSuccess ? MA_OK : MA_ERR_CUDA;
+  return launch_pdl(page_plan_kernel, dim3((unsigned)grid), dim3(kThreads), smem, st, p) == cudaSuccess ? MA_OK : MA_ERR_CUDA;
 }
 
 }  // namespace ma

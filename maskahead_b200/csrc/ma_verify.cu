@@ -230,6 +230,8 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant_
   const int b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const T* target = reinterpret_cast<const T*>(p.target) + (int64_t)b * p.st[0];
   const T* draft = p.draft == nullptr ? nullptr : reinterpret_cast<const T*>(p.draft) + (int64_t)b * p.sd[0];
+  pdl_wait();
+  pdl_launch_dependents();
   if (warp == 0) {       // the accepted run: the first refused draft, 32 at a time
     const int n = min(max(p.counts == nullptr ? p.K : p.counts[b], 0), p.K);
     int run = n;
@@ -359,8 +361,7 @@ int launch(const VerifyParams& p, cudaStream_t st) {
       return MA_ERR_CUDA;
     if (dev >= 0 && dev < 64) ready[dev] = true;
   }
-  verify_kernel<T><<<dim3(p.ctas, p.B), kThreads, kRingBytes, st>>>(p);
-  return cudaGetLastError() == cudaSuccess ? MA_OK : MA_ERR_CUDA;
+  return launch_pdl(verify_kernel<T>, dim3(p.ctas, p.B), dim3(kThreads), kRingBytes, st, p) == cudaSuccess ? MA_OK : MA_ERR_CUDA;
 }
 
 }  // namespace
