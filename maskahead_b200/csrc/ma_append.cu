@@ -13,9 +13,8 @@
 // lane. So the bf16 form does without divisions. With 8-bit significands a quotient a / s can
 // neither lie on nor within 2^-17 of a boundary of bf16 rounding (m s = a has no solution for a
 // 9-bit odd m), so a product with a reciprocal that is off by a few ulps rounds to the same
-// bf16. A key's divisor has 24 bits: there two products, with a reciprocal 2^-21 too large and
-// one as much too small, enclose the quotient, and where they round differently (one element
-// in 4000) it is divided.
+// bf16. A key's divisor has 24 bits: there the product, 2^-21 of it more and as much less, encloses
+// the quotient, and where the two ends round differently (one element in 4000) it is divided.
 #include <type_traits>
 
 #include "ma_kernels.cuh"
@@ -119,21 +118,25 @@ __device__ __forceinline__ Quantized quantize(const uint32_t x[kEach / 2]) {
   return r;
 }
 
-// A thread's divisors, and for bf16 rows their reciprocals, a little too large and too small.
+// A thread's divisors and, for bf16 rows, their reciprocals: in shared memory, a column per thread
+// (nobody else reads it), which leaves registers for half as many warps again.
 template <bool BF16>
 struct Divisors {
-  float kc[kEach], above[BF16 ? kEach : 1], below[BF16 ? kEach : 1];
+  static constexpr int kQuads = kEach / 4;
+  float4* column;          // [kQuads of kc, kQuads of 1 / kc][kThreads]
   bool usable;
+  __device__ __forceinline__ float4 kc(int quad) const { return column[quad * kThreads]; }
+  __device__ __forceinline__ float4 r(int quad) const { return column[(kQuads + quad) * kThreads]; }
   __device__ __forceinline__ void load(const float* p) {
     usable = true;
 #pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-      kc[e] = p[e];
+    for (int e = 0; e < kQuads; ++e) {
+      const float4 k = make_float4(p[4 * e], p[4 * e + 1], p[4 * e + 2], p[4 * e + 3]);
+      column[e * kThreads] = k;
       if (BF16) {
-        const float r = 1.0f / kc[e];
-        above[e] = r * (1.f + 4.76837158e-7f);
-        below[e] = r * (1.f - 4.76837158e-7f);
-        usable &= kc[e] > 1e-30f && kc[e] < 1e30f;
+        column[(kQuads + e) * kThreads] = make_float4(1.0f / k.x, 1.0f / k.y, 1.0f / k.z, 1.0f / k.w);
+        usable &= fminf(fminf(k.x, k.y), fminf(k.z, k.w)) > 1e-30f && fmaxf(fmaxf(k.x, k.y), fmaxf(k.z, k.w)) < 1e30f;
+        usable &= k.x == k.x && k.y == k.y && k.z == k.z && k.w == k.w;
       }
     }
   }
@@ -141,20 +144,34 @@ struct Divisors {
 
 __device__ __forceinline__ void divide(const Divisors<false>& k, float x[kEach]) {
 #pragma unroll
-  for (int e = 0; e < kEach; ++e) x[e] /= k.kc[e];
+  for (int e = 0; e < kEach / 4; ++e) {
+    const float4 d = k.kc(e);
+    x[4 * e] /= d.x;
+    x[4 * e + 1] /= d.y;
+    x[4 * e + 2] /= d.z;
+    x[4 * e + 3] /= d.w;
+  }
 }
+constexpr float kAbove = 1.f + 4.76837158e-7f, kBelow = 1.f - 4.76837158e-7f;     // 1 +- 2^-21
 __device__ __forceinline__ void divide(const Divisors<true>& k, uint32_t x[kEach / 2]) {
   uint32_t y[kEach / 2], apart = k.usable ? 0u : 1u;
 #pragma unroll
-  for (int e = 0; e < kEach / 2; ++e) {
-    const float a = lo_float(x[e]), b = hi_float(x[e]);
-    y[e] = bits(__floats2bfloat162_rn(a * k.above[2 * e], b * k.above[2 * e + 1]));
-    apart |= y[e] ^ bits(__floats2bfloat162_rn(a * k.below[2 * e], b * k.below[2 * e + 1]));
+  for (int e = 0; e < kEach / 4; ++e) {
+    const float4 r = k.r(e);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float a = lo_float(x[2 * e + i]) * (i ? r.z : r.x), b = hi_float(x[2 * e + i]) * (i ? r.w : r.y);
+      y[2 * e + i] = bits(__floats2bfloat162_rn(a * kAbove, b * kAbove));
+      apart |= y[2 * e + i] ^ bits(__floats2bfloat162_rn(a * kBelow, b * kBelow));
+    }
   }
   if (apart) {
 #pragma unroll
-    for (int e = 0; e < kEach / 2; ++e)
-      y[e] = bits(__floats2bfloat162_rn(lo_float(x[e]) / k.kc[2 * e], hi_float(x[e]) / k.kc[2 * e + 1]));
+    for (int e = 0; e < kEach / 4; ++e) {
+      const float4 d = k.kc(e);
+      y[2 * e] = bits(__floats2bfloat162_rn(lo_float(x[2 * e]) / d.x, hi_float(x[2 * e]) / d.y));
+      y[2 * e + 1] = bits(__floats2bfloat162_rn(lo_float(x[2 * e + 1]) / d.z, hi_float(x[2 * e + 1]) / d.w));
+    }
   }
 #pragma unroll
   for (int e = 0; e < kEach / 2; ++e) x[e] = y[e];
@@ -198,22 +215,33 @@ __device__ __forceinline__ void append_run(const AppendParams& p, int first, int
   __half* zero = reinterpret_cast<__half*>(const_cast<uint16_t*>(KEY ? p.kv.kz : p.kv.vz)) + sc0;
   const int64_t limit = (int64_t)p.kv.num_pages * p.kv.page_size;
 
+  __shared__ float4 sColumns[(KEY ? 2 : 0) * (kEach / 4) + 1][kThreads];
   Divisors<sizeof(T) == 2> kd;
+  kd.column = &sColumns[0][threadIdx.x];
   int held = -2;          // the request whose divisors are in kd
   Raw next[kRaw] = {};
   int64_t next_slot = -1;
   int next_seq = -1;
+  // pointers to the token that is fetched next, and the row that is written now
+  const T* x_at = src + first * stride;
+  const int64_t* slot_at = p.slots + first;
+  const int32_t* seq_at = p.seqs + first;
+  const int64_t x_step = step * stride, row_step = (int64_t)step * p.H * D;
+  int64_t row_at = ((int64_t)first * p.H + h) * D + c * kEach;
   auto fetch = [&](int i) {
     if (i < last) {
-      load_row(src + i * stride, next);
-      next_slot = p.slots[i];
-      next_seq = p.seqs[i];
+      load_row(x_at, next);
+      next_slot = *slot_at;
+      next_seq = *seq_at;
+      x_at += x_step;
+      slot_at += step;
+      seq_at += step;
     }
   };
   fetch(first);
   // the lanes of a row share its token, and every lane of a warp makes the same number of rounds
   const int rounds = __reduce_max_sync(0xffffffffu, (unsigned)(last > first ? (last - first + step - 1) / step : 0));
-  for (int k = 0, i = first; k < rounds; ++k, i += step) {
+  for (int k = 0, i = first; k < rounds; ++k, i += step, row_at += row_step) {
     Raw x[kRaw];
 #pragma unroll
     for (int e = 0; e < kRaw; ++e) x[e] = next[e];
@@ -235,28 +263,31 @@ __device__ __forceinline__ void append_run(const AppendParams& p, int first, int
       const float s = __half2float(q.step), z = __half2float(q.low);
       float back[kEach];
 #pragma unroll
-      for (int e = 0; e < kEach; ++e) {
-        back[e] = fmaf(q.code[e], s, z);
-        if (KEY) back[e] *= kd.kc[e];
+      for (int e = 0; e < kEach; ++e) back[e] = fmaf(q.code[e], s, z);
+      if (KEY) {
+#pragma unroll
+        for (int e = 0; e < kEach / 4; ++e) {
+          const float4 d = kd.kc(e);
+          back[4 * e] *= d.x;
+          back[4 * e + 1] *= d.y;
+          back[4 * e + 2] *= d.z;
+          back[4 * e + 3] *= d.w;
+        }
       }
       if (!owned) {
 #pragma unroll
         for (int e = 0; e < kEach; ++e) back[e] = 0.f;
       }
-      store_row(rows + ((int64_t)i * p.H + h) * D + c * kEach, back);
+      store_row(rows + row_at, back);
     }
     if (!owned || (uint64_t)slot >= (uint64_t)limit) continue;
-    int64_t page, at;
-    if (slot <= 0x7fffffffLL) {
-      page = p.page_div.div((int)slot);
-      at = slot - page * p.kv.page_size;
-    } else {
-      page = slot / p.kv.page_size;
-      at = slot - page * p.kv.page_size;
-    }
-    *reinterpret_cast<uint2*>(pay + page * sq[0] + at * sq[2]) = make_uint2(q.packed[0], q.packed[1]);
+    uint32_t page, at;                         // (a pool has fewer than 2^31 pages of fewer than 2^31 slots)
+    if (slot <= 0x7fffffffLL) page = (uint32_t)p.page_div.div((int)slot);
+    else page = (uint32_t)(slot / p.kv.page_size);
+    at = (uint32_t)(slot - (int64_t)page * p.kv.page_size);
+    *reinterpret_cast<uint2*>(pay + page * (uint64_t)sq[0] + at * (uint64_t)sq[2]) = make_uint2(q.packed[0], q.packed[1]);
     if (c % kPeers == 0) {
-      const int64_t o = page * sc[0] + at * sc[2];
+      const uint64_t o = page * (uint64_t)sc[0] + at * (uint64_t)sc[2];
       scale[o] = q.step;
       zero[o] = q.low;
     }

@@ -801,6 +801,7 @@ int ma_decode_attention(const ma_rows* q, const ma_kv* kv, int H, const ma_block
   if (!out || !so || !aligned16(out) || !strides16(so, 3, esize(q->dtype))) return MA_ERR_ARG;
   if (causal && cur->Tc > 0 && cur->Tc < q->T) return MA_ERR_ARG;
   if (q->dtype != MA_BF16 || kv->dtype != MA_BF16 || !packed_in_place(*kv, q->D)) return MA_ERR_UNSUPPORTED;
+  if ((int64_t)q->B * ((kv->nq + kDecodeUnit - 1) / kDecodeUnit + 1) > (1 << 30)) return MA_ERR_UNSUPPORTED;
   DecodeParams p;
   p.G = q->Hq / H;
   if ((int64_t)p.G * q->T > 0x7fffffffLL / 64) return MA_ERR_UNSUPPORTED;

@@ -178,10 +178,13 @@ __global__ void __launch_bounds__(kThreads) page_plan_kernel(const __grid_consta
 
   const int64_t step = (int64_t)gridDim.x * kThreads, first = (int64_t)blockIdx.x * kThreads + tid;
 
-  // ---- the tokens, four to a thread
-  const int64_t quads = ((int64_t)p.max_tokens + 3) / 4;
+  // ---- the tokens, four to a thread and a run of them to a warp, so that a lane's next four are
+  // mostly of the same request
+  const int64_t quads = ((int64_t)p.max_tokens + 3) / 4, all_warps = (int64_t)gridDim.x * kWarps;
+  const int64_t run = ((quads + all_warps - 1) / all_warps + 31) / 32 * 32, at_warp = (int64_t)blockIdx.x * kWarps + warp;
+  const int64_t run_end = min(quads, (at_warp + 1) * run);
   int b = -1;
-  for (int64_t qd = first; qd < quads; qd += step) {
+  for (int64_t qd = at_warp * run + lane; qd < run_end; qd += 32) {
     const int i0 = (int)(qd * 4);
     long long slot[4];
     int own[4], pos[4];

@@ -51,6 +51,9 @@ def _scratch(device: torch.device, purpose: str, nbytes: int, given: torch.Tenso
     if given is None:
         held = _SHARED.get((device.index, purpose))
         if held is None or held[2] < nbytes:       # (the shared workspace of a purpose only ever grows, and only here)
+            if torch.cuda.is_current_stream_capturing():     # its zero fill would be a node of the graph
+                raise RuntimeError(f"run the largest call once before capturing a graph: the shared '{purpose}' "
+                                   "workspace must exist")
             ws = _lib.workspace(device, purpose, nbytes)
             held = _SHARED[(device.index, purpose)] = (ws, ws.data_ptr(), ws.numel())
         return held[1], held[2]

@@ -384,6 +384,29 @@ def test_other_prefixes_take_the_general_route(kind):
     assert (got.double().cpu() - ref).norm() / ref.norm() < limit
 
 
+def test_a_cache_takes_the_general_route_too():
+    """float32 queries, and more rows than are read in place, over a paged cache."""
+    cache = _make(2, 2, 128, [200, 90], 32, seed=30)
+    for hq, t, dtype in ((8, 2, torch.float32), (80, 2, torch.bfloat16)):
+        q, kc, vc = _inputs(2, hq, 2, t, 128, t, seed=31)
+        ref, _ = _attend_ref(q, cache.prefix(), kc, vc)
+        out = cache.attend(q.to(dtype), kc.to(dtype), vc.to(dtype))
+        assert out.dtype == dtype
+        # k and v rounded to bf16 on this route: 2^-8 of each, as test_packed_fa's 2e-2
+        assert (out.double() - ref).norm() <= 2e-2 * ref.norm()
+
+
+def test_a_capture_needs_the_workspace_first(monkeypatch):
+    import maskahead_b200.serving as serving
+
+    cache = _make(1, 1, 64, [10], 16, seed=32)
+    q, _, _ = _inputs(1, 1, 1, 1, 64, 0, seed=32)
+    monkeypatch.setattr(serving, "_SHARED", {})
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError):
+        cache.attend(q)
+
+
 def test_streams_graphs_and_own_workspace():
     from maskahead_b200.serving import decode_workspace_bytes
 
@@ -659,6 +682,45 @@ def test_append_stores_what_the_quantizer_gives(N, H, D, page, dtype):
         # one fp32 fma, for keys one fp32 product, one rounding to the type
         eps = (2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -22)
         assert ((rows.double() - ref).abs() <= eps * ref.abs() + 2.0 ** -22 * (c.abs() + zz.abs()) * 4).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_append_extreme_rows(dtype):
+    """Non-finite, huge, tiny, equal and signed-zero rows, and divisors of every size, give the
+    quantizer's bytes: the short cuts for bf16 rows hold or step aside."""
+    from maskahead_b200.layouts import quantize_tokens
+    from maskahead_b200.serving import PagedCache
+
+    H, D = 2, 128
+    g = torch.Generator().manual_seed(12)
+    rows = [torch.randn(H, D, generator=g) * s for s in (1e-40, 1e-30, 1e-9, 1e-4, 1.0, 300.0, 1e10, 1e30, 3e38)]
+    mixed = torch.randn(H, D, generator=g)
+    for value, where in ((float("nan"), 3), (float("inf"), 40), (float("-inf"), 70), (1e38, 100)):
+        x = mixed.clone()
+        x[:, where] = value
+        rows.append(x)
+    both = mixed.clone()
+    both[:, 5], both[:, 6] = float("inf"), float("-inf")
+    zeros = torch.zeros(H, D)
+    zeros[:, ::2] = -0.0
+    steps = torch.arange(D).float().expand(H, D) % 16                     # codes that fall on whole numbers
+    halves = (torch.arange(D).float().expand(H, D) % 31) * 0.5            # and between them
+    rows += [both, zeros, torch.full((H, D), float("nan")), torch.full((H, D), 7.0), steps, halves, -steps, halves * 3e-3]
+    x = torch.stack(rows).to(dtype).to(DEV)
+    n = x.shape[0]
+    divisors = [1.0, 2.0, 3.0, 1e-20, 1e20, 1e-35, 1e35, 0.0, 1.9999999]
+    for d in divisors:
+        kchan = torch.full((1, H, D), d, device=DEV)
+        if d == 3.0:
+            kchan += torch.rand(1, H, D, generator=g).to(DEV)
+        cache = PagedCache.allocate(batch=1, heads=H, head_dim=D, num_pages=2, page_size=32, max_pages=2, kchan=kchan)
+        cache.append(x, x, torch.arange(n, device=DEV), torch.zeros(n, dtype=torch.int32, device=DEV))
+        kc = kchan.expand(n, H, D).contiguous()
+        want_k, want_v = quantize_tokens(x[:, :, None].contiguous(), kc), quantize_tokens(x[:, :, None].contiguous())
+        for got, want in zip((cache.kq, cache.ks, cache.kz, cache.vq, cache.vs, cache.vz), want_k + want_v):
+            a, b = got[0, :, :n].transpose(0, 1), want[:, :, 0]
+            same = (a.view(torch.int16) == b.view(torch.int16)) if a.dtype == torch.float16 else a == b
+            assert same.all(), f"divisor {d}: rows {sorted(set(torch.nonzero(~same)[:, 0].tolist()))}"
 
 
 def test_append_strides_empty_and_refusals():
