@@ -487,17 +487,49 @@ typedef struct ma_page_plan_args {
 MA_API size_t ma_page_plan_workspace(void);
 MA_API int ma_page_plan(const ma_page_plan_args* a, const int32_t* new_lens, void* workspace, size_t workspace_bytes,
                         void* stream);
-MA_API int ma_append_tokens(const ma_kv* pool, int B, int H, int D, const void* k, const void* v, int32_t dtype, int N,
-                            const int64_t sk[2], const int64_t sv[2], const int64_t* slots, const int32_t* seqs,
-                            void* k_rows, void* v_rows, void* stream);
+typedef struct ma_append_args {
+  const void* k;              /* [N, H, D], strides sk / sv over (token, head) */
+  const void* v;
+  const int64_t* slots;       /* [N] */
+  const int32_t* seqs;        /* [N] */
+  void* k_rows;               /* [N, H, D] contiguous, or NULL */
+  void* v_rows;
+  int64_t sk[2], sv[2];
+  int32_t N, dtype;
+  const ma_kv* pool;
+  int32_t B, H, D, reserved;  /* reserved: 0 */
+} ma_append_args;
+MA_API int ma_append_tokens(const ma_append_args* a, void* stream);
+typedef struct ma_decode_args {
+  const void* q;              /* [B, Hq, T, D], strides sq over (b, hq, t) */
+  const void* k;              /* the step's own keys and values [B, H, Tc, D] (Tc 0: unused) */
+  const void* v;
+  void* out;                  /* [B, Hq, T, D], strides so */
+  void* workspace;
+  size_t workspace_bytes;
+  int64_t sq[3], sk[3], sv[3], so[3];
+  const ma_kv* kv;
+  int32_t dtype, B, Hq, H, T, D, Tc, causal;
+  float scale;
+  int32_t reserved;           /* 0 */
+} ma_decode_args;
 MA_API size_t ma_decode_attention_workspace(int B, int H, int R, int D, int Tc);
-MA_API int ma_decode_attention(const ma_rows* q, const ma_kv* kv, int H, const ma_block* cur, float scale, int causal,
-                               void* out, const int64_t so[3], void* workspace, size_t workspace_bytes, void* stream);
+MA_API int ma_decode_attention(const ma_decode_args* a, void* stream);
+typedef struct ma_verify_args {
+  const void* target;         /* [B, K + 1, V], strides st over (request, position) */
+  const void* draft;          /* [B, K, V], strides sd, or NULL */
+  const int32_t* tokens;      /* [B, K] */
+  const int32_t* counts;      /* [B], or NULL */
+  const float* uniforms;      /* [B, K + 1] */
+  int32_t* accepted;          /* [B] */
+  int32_t* out;               /* [B, K + 1] */
+  void* workspace;
+  size_t workspace_bytes;
+  int64_t st[2], sd[2];
+  int32_t dtype, B, K, V;
+} ma_verify_args;
 MA_API size_t ma_verify_drafts_workspace(int B, int V);
-MA_API int ma_verify_drafts(const void* target, const void* draft, int32_t dtype, int B, int K, int V,
-                            const int64_t st[2], const int64_t sd[2], const int32_t* tokens, const int32_t* counts,
-                            const float* uniforms, int32_t* accepted, int32_t* out, void* workspace,
-                            size_t workspace_bytes, void* stream);
+MA_API int ma_verify_drafts(const ma_verify_args* a, void* stream);
 
 #ifdef __cplusplus
 }

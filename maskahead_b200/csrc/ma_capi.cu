@@ -791,42 +791,60 @@ size_t ma_decode_attention_workspace(int B, int H, int R, int D, int Tc) {
   return 512 + kDecodeTickets * sizeof(unsigned) + decode_partials(H, R, D, ml);
 }
 
-int ma_decode_attention(const ma_rows* q, const ma_kv* kv, int H, const ma_block* cur, float scale, int causal,
-                        void* out, const int64_t so[3], void* workspace, size_t workspace_bytes, void* stream) {
-  int rc = check_rows(q);
+int ma_decode_attention(const ma_decode_args* a, void* stream) {
+  if (!a || !a->kv) return MA_ERR_ARG;
+  ma_rows q;
+  q.q = a->q;
+  q.dtype = a->dtype;
+  q.B = a->B;
+  q.Hq = a->Hq;
+  q.T = a->T;
+  q.D = a->D;
+  ma_block cur;
+  cur.k = a->k;
+  cur.v = a->v;
+  cur.Tc = a->Tc;
+  for (int i = 0; i < 3; ++i) {
+    q.sq[i] = a->sq[i];
+    cur.sk[i] = a->sk[i];
+    cur.sv[i] = a->sv[i];
+  }
+  const ma_kv* kv = a->kv;
+  const int H = a->H;
+  int rc = check_rows(&q);
   if (rc) return rc;
-  if (H <= 0 || q->Hq % H) return MA_ERR_ARG;
-  if ((rc = check_kv(kv, q->D))) return rc;
-  if ((rc = check_block(cur, q, H))) return rc;
-  if (!out || !so || !aligned16(out) || !strides16(so, 3, esize(q->dtype))) return MA_ERR_ARG;
-  if (causal && cur->Tc > 0 && cur->Tc < q->T) return MA_ERR_ARG;
-  if (q->dtype != MA_BF16 || kv->dtype != MA_BF16 || !packed_in_place(*kv, q->D)) return MA_ERR_UNSUPPORTED;
-  if ((int64_t)q->B * ((kv->nq + kDecodeUnit - 1) / kDecodeUnit + 1) > (1 << 30)) return MA_ERR_UNSUPPORTED;
+  if (H <= 0 || q.Hq % H) return MA_ERR_ARG;
+  if ((rc = check_kv(kv, q.D))) return rc;
+  if ((rc = check_block(&cur, &q, H))) return rc;
+  if (!a->out || !aligned16(a->out) || !strides16(a->so, 3, esize(q.dtype))) return MA_ERR_ARG;
+  if (a->causal && cur.Tc > 0 && cur.Tc < q.T) return MA_ERR_ARG;
+  if (q.dtype != MA_BF16 || kv->dtype != MA_BF16 || !packed_in_place(*kv, q.D)) return MA_ERR_UNSUPPORTED;
+  if ((int64_t)q.B * ((kv->nq + kDecodeUnit - 1) / kDecodeUnit + 1) > (1 << 30)) return MA_ERR_UNSUPPORTED;
   DecodeParams p;
-  p.G = q->Hq / H;
-  if ((int64_t)p.G * q->T > 0x7fffffffLL / 64) return MA_ERR_UNSUPPORTED;
-  p.R = p.G * q->T;
+  p.G = q.Hq / H;
+  if ((int64_t)p.G * q.T > 0x7fffffffLL / 64) return MA_ERR_UNSUPPORTED;
+  p.R = p.G * q.T;
   DecodePlan d;
-  plan_decode(q->B, H, p.R, q->D, kv, d);
-  if ((int64_t)H * d.row_tiles > 65535 || (int64_t)q->B * H * d.row_tiles > (int64_t)kDecodeTickets)
+  plan_decode(q.B, H, p.R, q.D, kv, d);
+  if ((int64_t)H * d.row_tiles > 65535 || (int64_t)q.B * H * d.row_tiles > (int64_t)kDecodeTickets)
     return MA_ERR_UNSUPPORTED;
   size_t ml;
-  const size_t scratch = decode_partials(H, p.R, q->D, ml);
-  if (!workspace || workspace_bytes < 512 + kDecodeTickets * sizeof(unsigned) + scratch) return MA_ERR_WORKSPACE;
-  char* base = align256(workspace) + 256;
-  p.q = reinterpret_cast<const __nv_bfloat16*>(q->q);
+  const size_t scratch = decode_partials(H, p.R, q.D, ml);
+  if (!a->workspace || a->workspace_bytes < 512 + kDecodeTickets * sizeof(unsigned) + scratch) return MA_ERR_WORKSPACE;
+  char* base = align256(a->workspace) + 256;
+  p.q = reinterpret_cast<const __nv_bfloat16*>(q.q);
   p.kv = *kv;
-  p.cur = *cur;
-  p.B = q->B;
+  p.cur = cur;
+  p.B = q.B;
   p.H = H;
-  p.T = q->T;
-  p.D = q->D;
-  p.scale = scale;
-  p.causal = causal;
-  p.out = reinterpret_cast<__nv_bfloat16*>(out);
+  p.T = q.T;
+  p.D = q.D;
+  p.scale = a->scale;
+  p.causal = a->causal;
+  p.out = reinterpret_cast<__nv_bfloat16*>(a->out);
   for (int i = 0; i < 3; ++i) {
-    p.sq[i] = q->sq[i];
-    p.so[i] = so[i];
+    p.sq[i] = q.sq[i];
+    p.so[i] = a->so[i];
   }
   p.tickets = reinterpret_cast<unsigned*>(base);
   base += kDecodeTickets * sizeof(unsigned);
@@ -876,39 +894,38 @@ int ma_page_plan(const ma_page_plan_args* a, const int32_t* new_lens, void* work
   return launch_page_plan(p, (cudaStream_t)stream);
 }
 
-int ma_append_tokens(const ma_kv* pool, int B, int H, int D, const void* k, const void* v, int32_t dtype, int N,
-                     const int64_t sk[2], const int64_t sv[2], const int64_t* slots, const int32_t* seqs,
-                     void* k_rows, void* v_rows, void* stream) {
-  if (!pool || B <= 0 || H <= 0 || N < 0) return MA_ERR_ARG;
-  if (H > 65535) return MA_ERR_UNSUPPORTED;
-  if (D != 64 && D != 128) return MA_ERR_UNSUPPORTED;
-  if (!valid_dtype(dtype)) return MA_ERR_ARG;
+int ma_append_tokens(const ma_append_args* a, void* stream) {
+  if (!a || !a->pool || a->B <= 0 || a->H <= 0 || a->N < 0) return MA_ERR_ARG;
+  const ma_kv* pool = a->pool;
+  if (a->H > 65535) return MA_ERR_UNSUPPORTED;
+  if (a->D != 64 && a->D != 128) return MA_ERR_UNSUPPORTED;
+  if (!valid_dtype(a->dtype)) return MA_ERR_ARG;
   if (pool->layout != MA_KV_PACKED_TOKEN || pool->nf != 0) return MA_ERR_UNSUPPORTED;
   if (pool->page_size <= 0 || pool->num_pages <= 0 || pool->nq <= 0) return MA_ERR_ARG;
-  int rc = check_kv(pool, D);
+  int rc = check_kv(pool, a->D);
   if (rc) return rc;
-  if (N == 0) return MA_OK;
-  if (!k || !v || !sk || !sv || !slots || !seqs || !aligned16(k) || !aligned16(v)) return MA_ERR_ARG;
-  if (!strides16(sk, 2, esize(dtype)) || !strides16(sv, 2, esize(dtype))) return MA_ERR_ARG;
-  if ((k_rows && !aligned16(k_rows)) || (v_rows && !aligned16(v_rows))) return MA_ERR_ARG;
+  if (a->N == 0) return MA_OK;
+  if (!a->k || !a->v || !a->slots || !a->seqs || !aligned16(a->k) || !aligned16(a->v)) return MA_ERR_ARG;
+  if (!strides16(a->sk, 2, esize(a->dtype)) || !strides16(a->sv, 2, esize(a->dtype))) return MA_ERR_ARG;
+  if ((a->k_rows && !aligned16(a->k_rows)) || (a->v_rows && !aligned16(a->v_rows))) return MA_ERR_ARG;
   if (pool->skc[0] < 0 || pool->skc[1] < 0) return MA_ERR_ARG;
   AppendParams p;
-  p.k = k;
-  p.v = v;
+  p.k = a->k;
+  p.v = a->v;
   for (int i = 0; i < 2; ++i) {
-    p.sk[i] = sk[i];
-    p.sv[i] = sv[i];
+    p.sk[i] = a->sk[i];
+    p.sv[i] = a->sv[i];
   }
-  p.N = N;
-  p.B = B;
-  p.H = H;
-  p.D = D;
-  p.slots = slots;
-  p.seqs = seqs;
+  p.N = a->N;
+  p.B = a->B;
+  p.H = a->H;
+  p.D = a->D;
+  p.slots = a->slots;
+  p.seqs = a->seqs;
   p.kv = *pool;
-  p.k_rows = k_rows;
-  p.v_rows = v_rows;
-  return launch_append_tokens(p, dtype, (cudaStream_t)stream);
+  p.k_rows = a->k_rows;
+  p.v_rows = a->v_rows;
+  return launch_append_tokens(p, a->dtype, (cudaStream_t)stream);
 }
 
 size_t ma_verify_drafts_workspace(int B, int V) {
@@ -920,43 +937,43 @@ size_t ma_verify_drafts_workspace(int B, int V) {
   return 512 + kVerifyTickets * sizeof(unsigned) + (size_t)B * spans * sizeof(unsigned long long);
 }
 
-int ma_verify_drafts(const void* target, const void* draft, int32_t dtype, int B, int K, int V, const int64_t st[2],
-                     const int64_t sd[2], const int32_t* tokens, const int32_t* counts, const float* uniforms,
-                     int32_t* accepted, int32_t* out, void* workspace, size_t workspace_bytes, void* stream) {
-  if (B <= 0 || K < 0 || V <= 0 || !target || !st || !uniforms || !accepted || !out) return MA_ERR_ARG;
-  if (dtype != MA_F32 && dtype != MA_BF16 && dtype != MA_F16) return MA_ERR_ARG;
-  if (K > 0 && !tokens) return MA_ERR_ARG;
-  if (draft && K > 0 && (!sd || sd[0] < 0 || sd[1] < 0)) return MA_ERR_ARG;
-  if (st[0] < 0 || st[1] < 0) return MA_ERR_ARG;
-  const uintptr_t low = dtype == MA_F32 ? 3 : 1;
-  if ((reinterpret_cast<uintptr_t>(target) | reinterpret_cast<uintptr_t>(draft)) & low) return MA_ERR_ARG;
-  if (B > verify_max_requests() || V > (1 << 20)) return MA_ERR_UNSUPPORTED;
-  if (!workspace || workspace_bytes < ma_verify_drafts_workspace(B, V)) return MA_ERR_WORKSPACE;
-  VerifyParams p;
-  p.target = target;
-  p.draft = K > 0 ? draft : nullptr;
-  p.st[0] = st[0];
-  p.st[1] = st[1];
-  p.sd[0] = draft && K > 0 ? sd[0] : 0;
-  p.sd[1] = draft && K > 0 ? sd[1] : 0;
-  p.tokens = tokens;
-  p.counts = counts;
-  p.uniforms = uniforms;
-  p.B = B;
-  p.K = K;
-  p.V = V;
+int ma_verify_drafts(const ma_verify_args* a, void* stream) {
+  if (!a || a->B <= 0 || a->K < 0 || a->V <= 0 || !a->target || !a->uniforms || !a->accepted || !a->out) return MA_ERR_ARG;
+  if (a->dtype != MA_F32 && a->dtype != MA_BF16 && a->dtype != MA_F16) return MA_ERR_ARG;
+  if (a->K > 0 && !a->tokens) return MA_ERR_ARG;
+  if (a->draft && a->K > 0 && (a->sd[0] < 0 || a->sd[1] < 0)) return MA_ERR_ARG;
+  if (a->st[0] < 0 || a->st[1] < 0) return MA_ERR_ARG;
+  const uintptr_t low = a->dtype == MA_F32 ? 3 : 1;
+  if ((reinterpret_cast<uintptr_t>(a->target) | reinterpret_cast<uintptr_t>(a->draft)) & low) return MA_ERR_ARG;
+  if (a->B > verify_max_requests() || a->V > (1 << 20)) return MA_ERR_UNSUPPORTED;
   VerifyPlan plan;
-  plan_verify(B, V, dtype == MA_F32 ? 4 : 2, plan);
+  plan_verify(a->B, a->V, a->dtype == MA_F32 ? 4 : 2, plan);
+  if (!a->workspace || a->workspace_bytes < 512 + kVerifyTickets * sizeof(unsigned) +
+                                                (size_t)a->B * plan.spans * sizeof(unsigned long long))
+    return MA_ERR_WORKSPACE;
+  VerifyParams p;
+  p.target = a->target;
+  p.draft = a->K > 0 ? a->draft : nullptr;
+  for (int i = 0; i < 2; ++i) {
+    p.st[i] = a->st[i];
+    p.sd[i] = p.draft ? a->sd[i] : 0;
+  }
+  p.tokens = a->tokens;
+  p.counts = a->counts;
+  p.uniforms = a->uniforms;
+  p.B = a->B;
+  p.K = a->K;
+  p.V = a->V;
   p.ctas = plan.ctas;
   p.share = plan.share;
   p.per_warp = plan.per_warp;
   p.spans = plan.spans;
-  p.accepted = accepted;
-  p.out = out;
-  char* base = align256(workspace) + 256;
+  p.accepted = a->accepted;
+  p.out = a->out;
+  char* base = align256(a->workspace) + 256;
   p.tickets = reinterpret_cast<unsigned*>(base);
   p.sums = reinterpret_cast<unsigned long long*>(base + kVerifyTickets * sizeof(unsigned));
-  return launch_verify_drafts(p, dtype, (cudaStream_t)stream);
+  return launch_verify_drafts(p, a->dtype, (cudaStream_t)stream);
 }
 
 }  // extern "C"

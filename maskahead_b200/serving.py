@@ -21,12 +21,13 @@ tensor of decode_workspace_bytes / verify_workspace_bytes / PLAN_WORKSPACE_BYTES
 
 from __future__ import annotations
 
+import ctypes
 import functools
 
 import torch
 
 from . import _lib
-from ._lib import MaBlock, MaRows, i64
+from ._lib import APPEND_ARGS, DECODE_HEAD, DECODE_TAIL, VERIFY_ARGS
 from .layouts import Prefix, as_prefix, kv_descriptor
 
 __all__ = ["PagedCache", "TokenPlan", "decode_attention", "verify_drafts", "decode_workspace_bytes",
@@ -176,6 +177,7 @@ class PagedCache:
             if t.device != self.device:
                 raise ValueError("a cache's tensors must lie on one device")
         self._desc = kv_descriptor(self.prefix())       # checks types and strides
+        self._kv = ctypes.addressof(self._desc.kv)
         self._lib = _lib.lib()
         self._forms: dict[tuple, _Call] = {}            # attention calls' forms that passed their checks
 
@@ -229,11 +231,11 @@ class PagedCache:
         if return_rows:
             rows_k = torch.empty_like(k) if k.is_contiguous() else k.new_empty(shape)
             rows_v = torch.empty_like(rows_k)
-        rc = self._lib.ma_append_tokens(
-            self._desc.kv, self.batch, self.heads, self.head_dim, k.data_ptr(), v.data_ptr(), code, n,
-            _strides(k.stride()[:2]), _strides(v.stride()[:2]), slots.data_ptr(), seqs.data_ptr(),
-            rows_k.data_ptr() if return_rows else None, rows_v.data_ptr() if return_rows else None,
-            _lib.stream_handle(dev))
+        sk, sv = k.stride(), v.stride()
+        rc = self._lib.ma_append_tokens(APPEND_ARGS.pack(
+            k.data_ptr(), v.data_ptr(), slots.data_ptr(), seqs.data_ptr(), rows_k.data_ptr() if return_rows else 0,
+            rows_v.data_ptr() if return_rows else 0, sk[0], sk[1], sv[0], sv[1], n, code, self._kv, self.batch,
+            self.heads, self.head_dim, 0), _lib.stream_handle(dev))
         if rc:
             _lib.check("ma_append_tokens", rc)
         return (rows_k, rows_v) if return_rows else None
@@ -264,12 +266,6 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
     return t.clone(memory_format=torch.contiguous_format)
 
 
-@functools.lru_cache(maxsize=1024)
-def _strides(pair: tuple):
-    """Two strides as the C ABI takes them (never written to, so calls may share them)."""
-    return i64(*pair)
-
-
 # ----------------------------------------------------------------------------- attention
 def decode_attention(query: torch.Tensor, prefix, current_key: torch.Tensor | None = None,
                      current_value: torch.Tensor | None = None, *, scaling: float | None = None, causal: bool = True,
@@ -294,11 +290,10 @@ class _Call:
     """What one form of an in-place attention call (its tensors' shapes, strides and types)
     passes besides the pointers."""
 
-    __slots__ = ("run", "device", "heads", "geometry", "sq", "tc", "sk", "sv", "shape", "so", "scale", "causal", "nbytes", "packed")
+    __slots__ = ("run", "device", "block", "tail", "keep", "shape", "packed", "nbytes")
 
 
 _MAX_FORMS = 256     # remembered forms per cache; a loop has a few
-_NO_BLOCK = MaBlock()
 
 
 def _attend(query, source, desc, current_key, current_value, scaling, causal, out, workspace):
@@ -323,7 +318,7 @@ def _attend(query, source, desc, current_key, current_value, scaling, causal, ou
         q2 = _aligned(query)
         if q2 is not query or k2 is not current_key or v2 is not current_value:
             return _attend(q2, source, desc, k2, v2, scaling, causal, out, workspace)
-        call = _attend_form(query, source, current_key, current_value, scaling, causal, out)
+        call = _attend_form(query, source, desc, current_key, current_value, scaling, causal, out)
         if call is None:
             return _attend_general(query, source, current_key, current_value, scaling, causal, out)
         if forms is not None:
@@ -332,7 +327,7 @@ def _attend(query, source, desc, current_key, current_value, scaling, causal, ou
             forms[form] = call
     q = query.data_ptr()
     k = v = 0
-    if call.tc:
+    if call.block:
         k, v = current_key.data_ptr(), current_value.data_ptr()
     if (q | k | v) & 15:       # strides that can be read, but a start between 16-byte boundaries
         if k | v:
@@ -340,14 +335,10 @@ def _attend(query, source, desc, current_key, current_value, scaling, causal, ou
         return _attend(_aligned(query), source, desc, current_key, current_value, scaling, causal, out, workspace)
     if out is not None and out.data_ptr() & 15:
         raise ValueError("out must start on a 16-byte boundary")
-    if desc is None:
-        desc = kv_descriptor(source, batch=query.shape[0], heads=call.heads, head_dim=query.shape[3])
     o = out if out is not None else torch.empty_like(query) if call.packed else query.new_empty(call.shape)
     dev = call.device
     ws, nbytes = _scratch(dev, "decode", call.nbytes, workspace)
-    rc = call.run(MaRows(q, _lib.MA_BF16, *call.geometry, call.sq), desc.kv, call.heads,
-                  MaBlock(k, v, call.tc, call.sk, call.sv) if call.tc else _NO_BLOCK,
-                  call.scale, call.causal, o.data_ptr(), call.so, ws, nbytes, _lib.stream_handle(dev))
+    rc = call.run(DECODE_HEAD.pack(q, k, v, o.data_ptr(), ws, nbytes) + call.tail, _lib.stream_handle(dev))
     if rc == _lib.MA_ERR_UNSUPPORTED:
         return _attend_general(query, source, current_key, current_value, scaling, causal, out)
     if rc:
@@ -355,7 +346,7 @@ def _attend(query, source, desc, current_key, current_value, scaling, causal, ou
     return o
 
 
-def _attend_form(query, source, current_key, current_value, scaling, causal, out) -> _Call | None:
+def _attend_form(query, source, desc, current_key, current_value, scaling, causal, out) -> _Call | None:
     """Check a call; its _Call when it is read in place, None for the general route."""
     if query.ndim != 4:
         raise ValueError("query must have shape [B, Hq, T, D]")
@@ -390,15 +381,16 @@ def _attend_form(query, source, current_key, current_value, scaling, causal, out
     if query.dtype != torch.bfloat16 or rows > MAX_DECODE_ROWS or not (
             cached or (source.nq > 0 and source.nf == 0 and source.kmode == 1)):
         return None
+    if desc is None:
+        desc = kv_descriptor(source, batch=b, heads=heads, head_dim=d)
     call = _Call()
-    call.run, call.device = _lib.lib().ma_decode_attention, query.device
-    call.heads, call.geometry, call.tc = heads, (b, hq, t, d), tc
-    call.sq = i64(*query.stride()[:3])
-    call.sk, call.sv = (i64(*current_key.stride()[:3]), i64(*current_value.stride()[:3])) if tc else (i64(0, 0, 0), i64(0, 0, 0))
+    call.run, call.device, call.block, call.keep = _lib.lib().ma_decode_attention, query.device, tc > 0, desc
     call.shape, call.packed = (b, hq, t, d), query.is_contiguous()
-    call.so = i64(hq * t * d, t * d, d) if out is None else i64(*out.stride()[:3])
-    call.scale = d ** -0.5 if scaling is None else float(scaling)
-    call.causal = 1 if causal else 0
+    none = (0, 0, 0)
+    call.tail = DECODE_TAIL.pack(
+        *query.stride()[:3], *(current_key.stride()[:3] if tc else none), *(current_value.stride()[:3] if tc else none),
+        *((hq * t * d, t * d, d) if out is None else out.stride()[:3]), ctypes.addressof(desc.kv), _lib.MA_BF16, b, hq,
+        heads, t, d, tc, 1 if causal else 0, d ** -0.5 if scaling is None else float(scaling), 0)
     call.nbytes = int(_lib.lib().ma_decode_attention_workspace(b, heads, rows, d, tc))
     return call
 
@@ -454,11 +446,11 @@ def verify_drafts(target: torch.Tensor, draft: torch.Tensor | None, tokens: torc
     accepted = uniforms.new_empty(b, dtype=torch.int32) if counts is None else torch.empty_like(counts)
     out = tokens.new_empty((b, k1))
     ws, nbytes = _scratch(dev, "verify", verify_workspace_bytes(b, v), workspace)
-    rc = _lib.lib().ma_verify_drafts(
-        target.data_ptr(), None if draft is None else draft.data_ptr(), code, b, k, v, _strides(target.stride()[:2]),
-        None if draft is None else _strides(draft.stride()[:2]), tokens.data_ptr(),
-        None if counts is None else counts.data_ptr(), uniforms.data_ptr(), accepted.data_ptr(), out.data_ptr(), ws,
-        nbytes, _lib.stream_handle(dev))
+    st, sd = target.stride(), (0, 0) if draft is None else draft.stride()
+    rc = _lib.lib().ma_verify_drafts(VERIFY_ARGS.pack(
+        target.data_ptr(), 0 if draft is None else draft.data_ptr(), tokens.data_ptr(),
+        0 if counts is None else counts.data_ptr(), uniforms.data_ptr(), accepted.data_ptr(), out.data_ptr(), ws, nbytes,
+        st[0], st[1], sd[0], sd[1], code, b, k, v), _lib.stream_handle(dev))
     if rc:
         _lib.check("ma_verify_drafts", rc)
     return accepted, out

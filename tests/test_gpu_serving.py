@@ -432,8 +432,10 @@ def test_streams_graphs_and_own_workspace():
 
 
 def test_attention_refusals():
-    from maskahead_b200 import KernelUnavailableError, MaError
-    from maskahead_b200._lib import MaBlock, MaRows, i64, lib
+    import ctypes
+
+    from maskahead_b200 import KernelUnavailableError
+    from maskahead_b200._lib import DECODE_HEAD, DECODE_TAIL, lib
     from maskahead_b200.serving import PagedCache, decode_attention
 
     cache = _make(2, 2, 128, [50, 60], 16, seed=23)
@@ -465,17 +467,17 @@ def test_attention_refusals():
     with pytest.raises(ValueError):
         decode_attention(q, type("Empty", (), {"nq": 0, "kf": None, "nf": 0})())
     # the C entry itself
-    L = lib()
-    r = MaRows(q.data_ptr(), 1, 2, 4, 2, 128, tuple(q.stride()[:3]))
-    o = torch.empty_like(q)
-    so = i64(*o.stride()[:3])
-    kv = cache._desc.kv
-    assert L.ma_decode_attention(r, kv, 2, MaBlock(), 1.0, 1, o.data_ptr(), so, None, 0, None) == -3
-    assert L.ma_decode_attention(r, kv, 3, MaBlock(), 1.0, 1, o.data_ptr(), so, None, 0, None) == -1
-    r32 = MaRows(q.data_ptr(), 0, 2, 4, 2, 128, tuple(q.stride()[:3]))
-    assert L.ma_decode_attention(r32, kv, 2, MaBlock(), 1.0, 1, o.data_ptr(), so, None, 0, None) == -2
+    L, o = lib(), torch.empty_like(q)
+
+    def call(dtype=1, heads=2, tc=0, ptr=q.data_ptr(), ws=0, nbytes=0):
+        st = q.stride()[:3]
+        return L.ma_decode_attention(
+            DECODE_HEAD.pack(ptr, 0, 0, o.data_ptr(), ws, nbytes)
+            + DECODE_TAIL.pack(*st, *st, *st, *st, ctypes.addressof(cache._desc.kv), dtype, 2, 4, heads, 2, 128, tc, 1, 1.0, 0), None)
+
+    assert call() == -3 and call(heads=3) == -1 and call(dtype=0) == -2 and call(tc=2) == -1 and call(ptr=q.data_ptr() + 2) == -1
+    assert L.ma_decode_attention(None, None) == -1
     assert L.ma_decode_attention_workspace(0, 1, 1, 128, 0) == 0
-    assert MaError is not None
 
 
 # ------------------------------------------------------------------------- page plans

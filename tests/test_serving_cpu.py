@@ -18,21 +18,63 @@ def lib():
     return maskahead_b200.load_library()
 
 
-def test_rejected_arguments(lib):
-    from maskahead_b200._lib import MaBlock, MaKV, MaPagePlan, MaRows, i64
+def _append(pool=None, k=0, n=1, dtype=1, d=128):
+    from maskahead_b200._lib import APPEND_ARGS
 
-    s2, s3 = i64(0, 0), i64(0, 0, 0)
+    return APPEND_ARGS.pack(k, k, k, k, 0, 0, 128, 128, 128, 128, n, dtype, 0 if pool is None else ctypes.addressof(pool), 1, 1, d, 0)
+
+
+def _verify(target=16, vocab=8, dtype=0, ws=0, nbytes=0):
+    from maskahead_b200._lib import VERIFY_ARGS
+
+    return VERIFY_ARGS.pack(target, 16, 16, 0, 16, 16, 16, ws, nbytes, 0, 0, 0, 0, dtype, 1, 1, vocab)
+
+
+def test_rejected_arguments(lib):
+    from maskahead_b200._lib import DECODE_HEAD, DECODE_TAIL, MaKV, MaPagePlan
+
+    kv = MaKV()
     assert lib.ma_page_plan(MaPagePlan(), None, None, 0, None) == -1
     assert lib.ma_page_plan(None, 16, None, 0, None) == -1
-    assert lib.ma_append_tokens(MaKV(), 1, 1, 128, None, None, 1, 1, s2, s2, None, None, None, None, None) == -2     # not packed
-    assert lib.ma_append_tokens(None, 1, 1, 128, None, None, 1, 1, s2, s2, None, None, None, None, None) == -1
-    assert lib.ma_append_tokens(MaKV(), 1, 1, 96, None, None, 1, 1, s2, s2, None, None, None, None, None) == -2
-    assert lib.ma_decode_attention(MaRows(), MaKV(), 1, MaBlock(), 1.0, 1, None, s3, None, 0, None) == -1
-    assert lib.ma_verify_drafts(None, None, 0, 1, 1, 8, s2, s2, None, None, None, None, None, None, 0, None) == -1
-    # addresses that are never read: the vocabulary and the workspace are looked at first
-    assert lib.ma_verify_drafts(16, 16, 0, 1, 1, (1 << 20) + 1, s2, s2, 16, None, 16, 16, 16, None, 0, None) == -2
-    assert lib.ma_verify_drafts(16, 16, 0, 1, 1, 8, s2, s2, 16, None, 16, 16, 16, None, 0, None) == -3
-    assert lib.ma_verify_drafts(17, 16, 0, 1, 1, 8, s2, s2, 16, None, 16, 16, 16, None, 0, None) == -1
+    assert lib.ma_append_tokens(None, None) == -1
+    assert lib.ma_append_tokens(_append(), None) == -1
+    assert lib.ma_append_tokens(_append(kv), None) == -2              # a dense cache
+    assert lib.ma_append_tokens(_append(kv, d=96), None) == -2
+    assert lib.ma_append_tokens(_append(kv, dtype=2), None) == -1
+    assert lib.ma_decode_attention(None, None) == -1
+    assert lib.ma_decode_attention(DECODE_HEAD.pack(0, 0, 0, 0, 0, 0) + DECODE_TAIL.pack(*[0] * 12, ctypes.addressof(kv), *[1] * 8, 1.0, 0),
+                                   None) == -1
+    # addresses that are never read: sizes, alignment and the workspace are looked at first
+    assert lib.ma_verify_drafts(None, None) == -1
+    assert lib.ma_verify_drafts(_verify(target=0), None) == -1
+    assert lib.ma_verify_drafts(_verify(dtype=7), None) == -1
+    assert lib.ma_verify_drafts(_verify(target=17), None) == -1
+    assert lib.ma_verify_drafts(_verify(vocab=(1 << 20) + 1), None) == -2
+    assert lib.ma_verify_drafts(_verify(), None) == -3
+    assert lib.ma_verify_drafts(_verify(ws=4096, nbytes=1000), None) == -3
+
+
+def test_packed_structs_match_the_header(tmp_path):
+    """The packed argument structs have the sizes and offsets that a C compiler gives the header's."""
+    import shutil
+    import subprocess
+    from pathlib import Path
+
+    from maskahead_b200._lib import APPEND_ARGS, DECODE_HEAD, DECODE_TAIL, VERIFY_ARGS
+
+    cc = shutil.which("gcc") or shutil.which("cc")
+    if cc is None:
+        pytest.skip("no C compiler")
+    src, exe = tmp_path / "sizes.c", tmp_path / "sizes"
+    src.write_text('#include <stddef.h>\n#include <stdio.h>\n#include "maskahead_b200.h"\nint main(void) {\n'
+                   'printf("%zu %zu %zu %zu %zu %zu %zu", sizeof(ma_append_args), offsetof(ma_append_args, pool), '
+                   'sizeof(ma_decode_args), offsetof(ma_decode_args, sq), offsetof(ma_decode_args, scale), '
+                   'sizeof(ma_verify_args), offsetof(ma_verify_args, st)); return 0; }\n')
+    root = Path(__file__).resolve().parents[1]
+    subprocess.run([cc, "-I", str(root / "include"), str(src), "-o", str(exe)], check=True)
+    got = [int(x) for x in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()]
+    head, tail = DECODE_HEAD.size, DECODE_TAIL.size
+    assert got == [APPEND_ARGS.size, 88, head + tail, head, head + 12 * 8 + 8 + 8 * 4, VERIFY_ARGS.size, 72]
 
 
 def test_page_plan_struct_matches_the_header(lib):
