@@ -23,11 +23,11 @@ bool contiguous_tiles(const ma_kv& kv, int D) {
 
 // Rows per tile: a tile of more rows unpacks the codes fewer times, but 24 and 32 rows leave
 // registers for 8 warps an SM only. 32 requests x 8192 slots, 4 KV heads, D = 128 (D = 64), us:
-//   14 rows: 16 -> 60 (45), 24 -> 78 (51), 32 -> 99 (60)
-//   21 rows: 16 -> 98 (75), 24 -> 82 (53), 32 -> 103 (62)
-//   28 rows: 16 -> 99 (76), 24 -> 134 (88), 32 -> 109 (67)
-//   35 rows: 16 -> 150 (112), 24 -> 134 (88), 32 -> 176 (105)
-//   56 rows: 16 -> 197 (147), 24 -> 209 (140), 32 -> 180 (110)
+//   14 rows: 16 -> 60 (39), 24 -> 78 (51), 32 -> 99 (60)
+//   21 rows: 16 -> 98 (67), 24 -> 82 (53), 32 -> 103 (62)
+//   28 rows: 16 -> 99 (69), 24 -> 134 (89), 32 -> 109 (67)
+//   35 rows: 16 -> 150 (92), 24 -> 134 (89), 32 -> 176 (107)
+//   56 rows: 16 -> 197 (129), 24 -> 209 (140), 32 -> 180 (111)
 // The general form and the wide one have no 24-row tile.
 int rows_per_tile(int R, int D, bool has24) {
   if (R <= 8) return 8;
@@ -58,7 +58,7 @@ void plan_decode(int B, int H, int R, int D, const ma_kv* kv, DecodePlan& plan) 
       plan.row_tiles = tiles;
     }
   }
-  const int per_head = H * plan.row_tiles, resident = sms * (plan.wide ? 1 : plan.rows == 8 && plan.fast ? 3 : 2);
+  const int per_head = H * plan.row_tiles, resident = sms * (plan.wide ? 1 : plan.fast && (plan.rows == 8 || (plan.rows == 16 && D == 64)) ? 3 : 2);
   plan.ctas = resident > per_head ? resident / per_head : 1;
 }
 

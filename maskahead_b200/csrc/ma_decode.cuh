@@ -1055,7 +1055,9 @@ int launch_decode_d(const DecodeParams& p, int rows, bool wide, bool fast, cudaS
     return launch<D, 4, 8, 1, true>(p, st);
   }
   if (rows == 8) return launch<D, 1, 4, 3, true>(p, st);
-  if (rows == 16) return launch<D, 2, 4, 2, true>(p, st);
+  // 14 rows, 32 x 8192 slots, 4 KV heads: 3 CTAs an SM (168 registers) 39.5 us against 44.4 for 2 at D = 64; at
+  // D = 128, where that spills the running rows, 62.4 against 60.0
+  if (rows == 16) return launch<D, 2, 4, D == 64 ? 3 : 2, true>(p, st);
   if (rows == 24) return launch<D, 3, 4, 2, true>(p, st);
   return launch<D, 4, 4, 2, true>(p, st);
 }
