@@ -35,7 +35,10 @@ struct Quantized {
   float code[kEach];
 };
 
-// 32-bit rows: the quantizer's operations as they are.
+// 32-bit rows. A code is the quotient (x - min) / s rounded twice, to 24 bits and to a whole number; the
+// product with 1 / s is within 2^-18 of the former (two roundings of 2^-24 of at most 15.1, and the
+// quotient's own), so it rounds to the same code unless it lies that close to a half: then (one row
+// of 16 in 8000) the quotients are taken.
 __device__ __forceinline__ Quantized quantize(const float x[kEach]) {
   float mn = x[0], mx = x[0];
 #pragma unroll
@@ -52,11 +55,20 @@ __device__ __forceinline__ Quantized quantize(const float x[kEach]) {
   Quantized r;
 #pragma unroll
   for (int w = 0; w < kEach / 8; ++w) r.packed[w] = 0u;
+  const float rs = 1.0f / s;
+  bool close = false;
 #pragma unroll
   for (int e = 0; e < kEach; ++e) {
-    r.code[e] = fminf(fmaxf(rintf((x[e] - mn) / s), 0.f), 15.f);
-    r.packed[e / 8] |= (uint32_t)r.code[e] << (4 * (e & 7));
+    const float t = (x[e] - mn) * rs, c = rintf(t);
+    close |= fabsf(t - c) >= 0.5f - 3.81469727e-6f;
+    r.code[e] = fminf(fmaxf(c, 0.f), 15.f);
   }
+  if (close) {
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) r.code[e] = fminf(fmaxf(rintf((x[e] - mn) / s), 0.f), 15.f);
+  }
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) r.packed[e / 8] |= (uint32_t)r.code[e] << (4 * (e & 7));
   r.step = __float2half_rn(s);
   r.low = __float2half_rn(mn);
   return r;

@@ -725,6 +725,27 @@ def test_append_extreme_rows(dtype):
             assert same.all(), f"divisor {d}: rows {sorted(set(torch.nonzero(~same)[:, 0].tolist()))}"
 
 
+def test_append_32_bit_rows_between_codes():
+    """Elements a few units in the last place from the middle between two codes get the quantizer's."""
+    from maskahead_b200.layouts import quantize_tokens
+    from maskahead_b200.serving import PagedCache
+
+    H, D, N = 2, 128, 4096
+    g = torch.Generator().manual_seed(21)
+    low, step = torch.randn(N, H, 4, 1, generator=g), 10.0 ** (3 * torch.rand(N, H, 4, 1, generator=g) - 2)
+    x = low + step * (torch.randint(0, 15, (N, H, 4, 32), generator=g) + 0.5)
+    x = x * (1 + torch.randint(-3, 4, x.shape, generator=g) * 2.0 ** -23)
+    x[..., 0], x[..., 1] = low[..., 0], (low + 15 * step)[..., 0]
+    x = x.reshape(N, H, D).to(DEV)
+    cache = PagedCache.allocate(batch=1, heads=H, head_dim=D, num_pages=N // 64, page_size=64, max_pages=N // 64,
+                                kchan=torch.ones(1, H, D, device=DEV))
+    cache.append(x, x, torch.arange(N, device=DEV), torch.zeros(N, dtype=torch.int32, device=DEV))
+    want = quantize_tokens(x[:, :, None].contiguous())
+    for got in ((cache.kq, cache.ks, cache.kz), (cache.vq, cache.vs, cache.vz)):
+        for a, b in zip(got, want):
+            assert torch.equal(a.transpose(1, 2).reshape(b[:, :, 0].shape), b[:, :, 0])
+
+
 def test_append_strides_empty_and_refusals():
     from maskahead_b200.serving import PagedCache
 
