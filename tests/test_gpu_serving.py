@@ -912,6 +912,37 @@ def test_verify_strides_and_determinism():
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_verify_rows_at_every_offset(dtype):
+    """Rows that begin at any element of 16 bytes, p's and q's apart, their mass where the summed
+    pieces begin and end (multiples of 512 elements and their neighbours)."""
+    from maskahead_b200.serving import verify_drafts
+
+    B, K, V = 24, 1, 4601
+    g = torch.Generator().manual_seed(31)
+    edge = torch.arange(V) % 512
+    heavy = (edge <= 1) | (edge >= 510) | (torch.arange(V) == V - 1)
+    p = (torch.rand(B, K + 1, V, generator=g) * torch.where(heavy, 0.05, 1e-6)).to(dtype).to(DEV)
+    q = (torch.rand(B, K, V, generator=g) * torch.where(heavy, 0.03, 1e-6)).to(dtype).to(DEV)
+    tokens = torch.randint(0, V, (B, K), generator=g).to(torch.int32).to(DEV)
+    u = torch.rand(B, K + 1, generator=g).to(DEV)
+    u[::2, 0] = 1.0 - 2.0 ** -24                          # every second draft refused, the others mostly accepted
+    u[1::2, 0] = 0.0
+    want = {}
+    for po in range(8):
+        for qo in range(8):
+            if po and qo and (po + 3 * qo) % 5:           # all pairs of parities, each offset at least twice
+                continue
+            wp = torch.full((B, K + 1, V + 15), float("nan"), device=DEV, dtype=dtype)
+            wq = torch.full((B, K, V + 15), float("nan"), device=DEV, dtype=dtype)
+            wp[..., po:po + V], wq[..., qo:qo + V] = p, q
+            for d in (wq[..., qo:qo + V], None):
+                if (d is None) not in want:
+                    want[d is None] = _verify_ref(p, None if d is None else q, tokens, None, u)
+                acc, out = verify_drafts(wp[..., po:po + V], d, tokens, None, u)
+                assert acc.tolist() == want[d is None][0] and out.tolist() == want[d is None][1], (po, qo)
+
+
 def test_verify_leaves_the_target_distribution():
     """Emitted first tokens are distributed as the target's row, whatever the drafter: 40000
     independent requests, each token's frequency within 5 standard deviations."""
