@@ -455,8 +455,8 @@ MA_API int ma_prefix_attention_gather(const ma_rows* q, const ma_kv* kv, int H, 
  *   to bf16 on the way, and over the step's own keys: with `causal`, row t sees block key
  *   j iff j <= t + Tc - T (Tc >= T), else every block key. A row without any key is zero.
  *   bf16 rows; scale and zero rows aligned to their D/16 bytes; other layouts return
- *   MA_ERR_UNSUPPORTED (ma_prefix_attention serves them). Any R = G*T, 32 rows per pass over
- *   the cache.
+ *   MA_ERR_UNSUPPORTED (ma_prefix_attention serves them). Any R = G*T, up to 32 rows per pass
+ *   over the cache.
  * ma_verify_drafts: K drafted tokens per request (tokens [B, K] contiguous, counts [B] of them
  *   in use, NULL = K) against the target's probabilities target [B, K + 1, V] and the
  *   drafter's draft [B, K, V] (strides over (request, position), vocabulary contiguous;

@@ -9,6 +9,8 @@ on top:
   maskahead_b200.hotpath   fast_step0, compact_attention, probe_attention,
                            value_score, lookahead_survivors
   maskahead_b200.layouts   LayerCacheView, Prefix, the ma_kv descriptor
+  maskahead_b200.serving   PagedCache, TokenPlan, decode_attention, verify_drafts: a
+                           decoding step over a paged k4v4 cache
 
 Kernel waits are bounded; ``device_status()`` raises ``MaError`` (MA_ERR_TIMEOUT) when one
 gave up since the last check. There is no CPU path: the operators need the built library

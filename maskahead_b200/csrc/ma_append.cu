@@ -15,6 +15,11 @@
 // 9-bit odd m), so a product with a reciprocal that is off by a few ulps rounds to the same
 // bf16. A key's divisor has 24 bits: there the product, 2^-21 of it more and as much less, encloses
 // the quotient, and where the two ends round differently (one element in 4000) it is divided.
+// 32-bit rows divide keys by their divisors, whose quotients they need to the last bit.
+//
+// Measured, with values out: 131000 tokens of 4 x 128 in bf16 146 us (622 MB: 4.3 TB/s, 66% of a copy's
+// rate; 125 us into consecutive slots, 103 us for a copy of as many bytes), 60000 in 32 bits 110 us (531 MB,
+// 4.8 TB/s); 13 tokens 3.2 us, the launch.
 #include <type_traits>
 
 #include "ma_kernels.cuh"

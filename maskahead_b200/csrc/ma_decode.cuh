@@ -10,21 +10,28 @@
 // c * 2^-24 (or c * 2^-20 from the high nibble), exact for the fp16 MMA; one shift and four
 // masks turn a 32-bit word into the A operands of eight codes.
 //
-// Bound: HBM (160 B per slot and KV head at D = 128) while the rows fit one or two 8-column
-// MMA tiles, the issue slots beyond. The rows are the N side (8 columns) of m16n8k16, the slots
-// (scores) or channels (output) its M side: G = 7 single-token rows waste one column of eight,
-// where a 128-row tcgen05 tile would waste 121 of 128 and need the codes written back to
-// shared memory as 16-bit operands first, 3.2 times their stored size.
+// Bound: HBM (160 B per slot and KV head at D = 128) while the rows fit one 8-column MMA tile, the
+// products' latency beyond (two warps a scheduler hold the running rows). The rows are the N side (8
+// columns) of m16n8k16, the slots (scores) or channels (output) its M side: G = 7 single-token
+// rows waste one column of eight, where 128 rows of a tcgen05 tile would waste 121. With the
+// slots as a tcgen05 tile's 128 rows instead, every code has to become a 16-bit operand in tensor
+// or shared memory first (13 instructions a word of codes against 5 here): that form was built, and
+// took 98 us against 60 at 14 rows and 140 against 134 at 35 (32 requests x 8192 slots, 4 KV heads,
+// D = 128).
+//
+// Measured, D = 128, 4 KV heads: 64 requests of 4096 to 16384 slots, 7 rows, 89 us (421 MB: 4.7 TB/s, 73%
+// of a copy's rate); 32 such requests, 35 rows, 168 us; 1 request, 8192 slots, 10.8 us, of which the
+// chain lengths -> page table -> tiles -> merge takes all but a microsecond or two.
 //
 // A warp owns 32-slot tiles and a private ring of shared memory filled by cp.async (16-byte
 // payload pieces in an XOR swizzle that ldmatrix reads without conflicts, scale and zero
 // blocks as they lie), so the main loop has no CTA barrier.
 //
-// Split: the live slots of all sequences, in units of 256, are one line that the CTAs of a
-// (head, row tile) cut into equal ranges -- from the lengths on the device, which the host does
-// not know -- so a ragged batch fills exactly one wave of resident CTAs. A range may end one
-// sequence and begin the next; a sequence cut by ranges leaves fp32 partials that the last of
-// its CTAs to arrive merges in a fixed order. Nobody waits.
+// Split: the live slots of all sequences, in units of 256, are cut from the lengths on the device
+// (which the host does not know) into whole shares of sequences where those balance, else, as one
+// line, into equal ranges that may end one sequence and begin the next; so a ragged batch fills one
+// wave of resident CTAs. A sequence cut into several leaves fp32 partials that the last of its CTAs to
+// arrive merges in a fixed order. Nobody waits.
 #pragma once
 
 #include "ma_kernels.cuh"

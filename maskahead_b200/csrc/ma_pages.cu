@@ -12,6 +12,9 @@
 // then expands its share of the tokens and table entries, so one launch does without a wait
 // between CTAs: the only thing a CTA must not do is overwrite lengths that another has yet to
 // read, so the CTA that arrives last at the ticket, after its reads, writes them.
+//
+// Measured: 8 requests by a token each 4.8 us, 256 by 2 to 16 8.0 us (the scan's and the page look-ups'
+// latency), 600 prompts of 1 to 16384 tokens 22.4 us (74 MB: 3.3 TB/s; the scan is 4 us of it).
 #include "ma_kernels.cuh"
 
 namespace ma {
