@@ -28,7 +28,7 @@ bool contiguous_tiles(const ma_kv& kv, int D) {
 //   28 rows: 16 -> 99 (69), 24 -> 134 (89), 32 -> 109 (67)
 //   35 rows: 16 -> 150 (92), 24 -> 134 (89), 32 -> 176 (107)
 //   56 rows: 16 -> 197 (129), 24 -> 209 (140), 32 -> 180 (111)
-// The general form and the wide one have no 24-row tile.
+// The general form has no 24-row tile.
 int rows_per_tile(int R, int D, bool has24) {
   if (R <= 8) return 8;
   if (R <= 16) return 16;
@@ -47,18 +47,25 @@ void plan_decode(int B, int H, int R, int D, const ma_kv* kv, DecodePlan& plan) 
   plan.rows = rows_per_tile(R, D, plan.fast);
   plan.row_tiles = (R + plan.rows - 1) / plan.rows;
   if (kv != nullptr) {
-    // few units by the cache's capacity (the lengths are on the device) and few sequences: the wide
-    // form. 1 x 32768 slots: 15 us against 24; 4 x 16384: 18 against 20; 16 x 8192 (2048 units):
-    // 27 both; 64 x 1024 (256 sequence heads): 24 against 16.
-    const int rows = rows_per_tile(R, D, false), tiles = (R + rows - 1) / rows;
-    const int64_t heads = (int64_t)B * H * tiles, units = heads * ((kv->nq + kDecodeUnit - 1) / kDecodeUnit);
-    if (heads <= sms && units <= 8 * sms) {
+    // The wide form for few sequences and few units of slots by the cache's capacity (the lengths are on the
+    // device), with the smallest tile of 8 or 16 rows that keeps to that: a tile's rows, not its slots, are
+    // what a short call waits for. D = 128, us, wide 8 / 16 / 32 rows and the other form: 4 requests of up to 3227
+    // slots, 2 heads, 64 rows 14 / 16 / 26 and 36; 1 x 8192, 4 heads, 21 rows 12 / 16 / 23 and 28; 1 x 39, 56 rows
+    // 8 / 11 / 18 and 21; 16 of up to 3000, 2 heads, 32 rows (10 units an SM at 8 rows) 24 / 18. Beyond 8 units an SM
+    // three 16-row tiles are still faster so (4 x 8192, 35 rows: 27 against 35; 56 rows: 38 against 49), one
+    // or two are not (10 x 8192, 14 rows: 30 against 25; 8 x 8192, 21 rows: 36 against 35). More sequence heads
+    // than SMs: 64 x 1000, 14 rows, 32 against 22.
+    for (int rows = 8; rows <= 16 && !plan.wide; rows *= 2) {
+      const int tiles = (R + rows - 1) / rows, most = rows == 16 && tiles >= 3 ? 16 : 8;
+      const int64_t heads = (int64_t)B * H * tiles, units = heads * ((kv->nq + kDecodeUnit - 1) / kDecodeUnit);
+      if (heads > sms || units > (int64_t)most * sms) continue;
       plan.wide = true;
       plan.rows = rows;
       plan.row_tiles = tiles;
     }
   }
-  const int per_head = H * plan.row_tiles, resident = sms * (plan.wide ? 1 : plan.fast && (plan.rows == 8 || (plan.rows == 16 && D == 64)) ? 3 : 2);
+  const bool three = plan.fast && (plan.rows == 8 || (plan.rows == 16 && D == 64));       // CTAs an SM, as launch_decode_d has them
+  const int per_head = H * plan.row_tiles, resident = sms * (plan.wide ? 1 : three ? 3 : 2);
   plan.ctas = resident > per_head ? resident / per_head : 1;
 }
 

@@ -1052,16 +1052,14 @@ template <int D>
 int launch_decode_d(const DecodeParams& p, int rows, bool wide, bool fast, cudaStream_t st) {
   if (!fast) {
     if (wide && rows == 8) return launch<D, 1, 8, 1, false>(p, st);
-    if (wide && rows == 16) return launch<D, 2, 8, 1, false>(p, st);
-    if (wide) return launch<D, 4, 8, 1, false>(p, st);
+    if (wide) return launch<D, 2, 8, 1, false>(p, st);
     if (rows == 8) return launch<D, 1, 4, 2, false>(p, st);
     if (rows == 16) return launch<D, 2, 4, 2, false>(p, st);
     return launch<D, 4, 4, 2, false>(p, st);
   }
   if (wide) {
     if (rows == 8) return launch<D, 1, 8, 1, true>(p, st);
-    if (rows == 16) return launch<D, 2, 8, 1, true>(p, st);
-    return launch<D, 4, 8, 1, true>(p, st);
+    return launch<D, 2, 8, 1, true>(p, st);
   }
   if (rows == 8) return launch<D, 1, 4, 3, true>(p, st);
   // 14 rows, 32 x 8192 slots, 4 KV heads: 3 CTAs an SM (168 registers) 39.5 us against 44.4 for 2 at D = 64; at
