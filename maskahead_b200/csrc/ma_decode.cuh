@@ -319,11 +319,12 @@ __device__ __forceinline__ void finish(const DecodeParams& p, const Segment& s, 
   merge_partials<D, ROWS, W>(p, s, b, h, r0, rows, ml, acc, buf, cap);
 }
 
-// The step's own keys, in fp32 on the CUDA cores: a warp per row, a lane per D/32 channels. Its
-// few keys stay in L1; as bf16 MMA tiles they would need a path of their own.
+// The step's own keys, in fp32 on the CUDA cores: a warp per up to four rows at once (their loads and
+// sums overlap: with one at a time a short request waited longer here than for its cache), a lane per
+// D/32 channels. Its few keys stay in L1; as bf16 MMA tiles they would need a path of their own.
 template <int D, int ROWS, int W>
 __device__ void block_rows(const DecodeParams& p, int b, int h, int r0, int rows, float* sRows, float2* sML) {
-  constexpr int kPad = D + 4, kCh = D / 32;
+  constexpr int kPad = D + 4, kCh = D / 32, kR = ROWS / W < 1 ? 1 : ROWS / W > 4 ? 4 : ROWS / W;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const __nv_bfloat16* K = reinterpret_cast<const __nv_bfloat16*>(p.cur.k) + (int64_t)b * p.cur.sk[0] + (int64_t)h * p.cur.sk[1] + lane * kCh;
   const __nv_bfloat16* V = reinterpret_cast<const __nv_bfloat16*>(p.cur.v) + (int64_t)b * p.cur.sv[0] + (int64_t)h * p.cur.sv[1] + lane * kCh;
@@ -339,45 +340,76 @@ __device__ void block_rows(const DecodeParams& p, int b, int h, int r0, int rows
     }
   };
 #pragma unroll 1
-  for (int r = warp; r < rows; r += W) {
-    const int g = (r0 + r) / p.T, t = (r0 + r) - g * p.T;
-    const int seen = p.causal ? min(p.cur.Tc, t + p.cur.Tc - p.T + 1) : p.cur.Tc;    // its first `seen` keys
-    float q[kCh], o[kCh], m = -INFINITY, l = 0.f;
-    load(p.q + (int64_t)b * p.sq[0] + (int64_t)(h * p.G + g) * p.sq[1] + (int64_t)t * p.sq[2] + lane * kCh, q);
+  for (int first = warp; first < rows; first += W * kR) {
+    int seen[kR], most = 0;          // a row sees the block's first `seen` keys
+    float q[kR][kCh], o[kR][kCh], m[kR], l[kR];
 #pragma unroll
-    for (int c = 0; c < kCh; ++c) o[c] = 0.f;
+    for (int i = 0; i < kR; ++i) {
+      const int r = min(first + W * i, rows - 1);      // (rows past the last: the last once more)
+      const int g = (r0 + r) / p.T, t = (r0 + r) - g * p.T;
+      seen[i] = p.causal ? min(p.cur.Tc, t + p.cur.Tc - p.T + 1) : p.cur.Tc;
+      most = max(most, seen[i]);
+      load(p.q + (int64_t)b * p.sq[0] + (int64_t)(h * p.G + g) * p.sq[1] + (int64_t)t * p.sq[2] + lane * kCh, q[i]);
+      m[i] = -INFINITY;
+      l[i] = 0.f;
+#pragma unroll
+      for (int c = 0; c < kCh; ++c) o[i][c] = 0.f;
+    }
 #pragma unroll 1
-    for (int j0 = 0; j0 < seen; j0 += 32) {
-      const int nj = min(32, seen - j0);
-      float sc = -INFINITY;
+    for (int j0 = 0; j0 < most; j0 += 32) {
+      const int nj = min(32, most - j0);
+      float v[kCh], pr[kR];
+      load(V + (int64_t)j0 * p.cur.sv[2], v);          // with the first key, not after its score
+#pragma unroll
+      for (int i = 0; i < kR; ++i) pr[i] = -INFINITY;
 #pragma unroll 2
       for (int j = 0; j < nj; ++j) {
-        float k[kCh], dot = 0.f;
+        float k[kCh];
         load(K + (int64_t)(j0 + j) * p.cur.sk[2], k);
 #pragma unroll
-        for (int c = 0; c < kCh; ++c) dot = fmaf(q[c], k[c], dot);
-        dot = warp_sum(dot);
-        if (lane == j) sc = dot * p.scale * kLog2e;
+        for (int i = 0; i < kR; ++i) {
+          float dot = 0.f;
+#pragma unroll
+          for (int c = 0; c < kCh; ++c) dot = fmaf(q[i][c], k[c], dot);
+          dot = warp_sum(dot);
+          if (lane == j && j0 + j < seen[i]) pr[i] = dot * p.scale * kLog2e;
+        }
       }
-      const float mn = fmaxf(m, warp_max(sc));
-      const float ms = mn == -INFINITY ? 0.f : mn;
-      const float corr = ex2(m - ms), pr = ex2(sc - ms);
-      m = mn;
-      l = l * corr + warp_sum(pr);
 #pragma unroll
-      for (int c = 0; c < kCh; ++c) o[c] *= corr;
-#pragma unroll 2
+      for (int i = 0; i < kR; ++i) {
+        const float mn = fmaxf(m[i], warp_max(pr[i]));
+        const float ms = mn == -INFINITY ? 0.f : mn;
+        const float corr = ex2(m[i] - ms);
+        pr[i] = ex2(pr[i] - ms);
+        m[i] = mn;
+        l[i] = l[i] * corr + warp_sum(pr[i]);
+#pragma unroll
+        for (int c = 0; c < kCh; ++c) o[i][c] *= corr;
+      }
+#pragma unroll 1
       for (int j = 0; j < nj; ++j) {
-        float v[kCh];
-        load(V + (int64_t)(j0 + j) * p.cur.sv[2], v);
-        const float w = __shfl_sync(0xffffffffu, pr, j);
+        float next[kCh];
+        load(V + (int64_t)min(j0 + j + 1, most - 1) * p.cur.sv[2], next);
 #pragma unroll
-        for (int c = 0; c < kCh; ++c) o[c] = fmaf(w, v[c], o[c]);
+        for (int i = 0; i < kR; ++i) {
+          const float w = __shfl_sync(0xffffffffu, pr[i], j);
+          if (j0 + j < seen[i]) {      // what a row does not see is not multiplied: it may be NaN
+#pragma unroll
+            for (int c = 0; c < kCh; ++c) o[i][c] = fmaf(w, v[c], o[i][c]);
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < kCh; ++c) v[c] = next[c];
       }
     }
 #pragma unroll
-    for (int c = 0; c < kCh; ++c) sRows[r * kPad + lane * kCh + c] = o[c];
-    if (lane == 0) sML[r] = make_float2(m, l);
+    for (int i = 0; i < kR; ++i) {
+      const int r = first + W * i;
+      if (r >= rows) break;
+#pragma unroll
+      for (int c = 0; c < kCh; ++c) sRows[r * kPad + lane * kCh + c] = o[i][c];
+      if (lane == 0) sML[r] = make_float2(m[i], l[i]);
+    }
   }
 }
 

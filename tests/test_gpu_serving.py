@@ -192,6 +192,19 @@ def test_decode_attention_blocks(Tc, T, causal):
     _close(out, ref, tol)
 
 
+@pytest.mark.parametrize("D,G,T,Tc", [(128, 7, 2, 2), (128, 3, 5, 40), (64, 8, 4, 4), (128, 1, 1, 1)])
+def test_block_keys_a_row_does_not_see(D, G, T, Tc):
+    """Later keys of the block may hold anything, NaN included."""
+    cache = _make(2, 2, D, [70, 0], 32, seed=40)
+    q, kc, vc = _inputs(2, 2 * G, 2, T, D, Tc, seed=41)
+    for t in range(T):
+        k, v = kc.clone(), vc.clone()
+        k[:, :, t + Tc - T + 1:], v[:, :, t + Tc - T + 1:] = float("nan"), float("nan")
+        out = cache.attend(q, k, v)
+        ref, tol = _attend_ref(q[:, :, :t + 1], cache.prefix(), kc[:, :, :t + Tc - T + 1], vc[:, :, :t + Tc - T + 1])
+        _close(out[:, :, :t + 1], ref, tol)
+
+
 def test_rows_without_a_key_are_zero():
     cache = _make(3, 2, 128, [0, 5, 0], 16, seed=6)
     q, _, _ = _inputs(3, 14, 2, 1, 128, 0, seed=6)
