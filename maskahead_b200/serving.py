@@ -36,10 +36,12 @@ __all__ = ["PagedCache", "TokenPlan", "decode_attention", "verify_drafts", "deco
 PLAN_WORKSPACE_BYTES = 512
 
 # Rows per KV head (query heads of the group x tokens) up to which attention reads the packed
-# cache in place; beyond, a prefix is unpacked once and the 128-row tensor-core tiles run.
-# 32 requests x 8192 slots, 4 KV heads, in place against unpacked: 7 rows 45 / 330 us, 35 rows
-# 135 / 562, 63 rows 184 / 564, 112 rows 374 / 331; one request: 12 / 29, 17 / 35, 30 / 36, 37 / 29.
-MAX_DECODE_ROWS = 64
+# cache in place; beyond, a prefix is unpacked once and the 128-row tensor-core tiles run. In
+# place against unpacked, device us: 32 requests x 8192 slots, 4 KV heads, 35 rows 134 / 562, 63
+# rows 178 / 564, 84 rows 280 / 567, 112 rows 374 / 331; 30 x 16000, 1 head, 96 rows 132 / 157; 4 x 8192, 4
+# heads, 112 rows 71 / 58; 1 x 8192, 35 rows 14 / 35, 84 rows 19 / 35, 112 rows 22 / 28 (and the unpacked
+# route's host time is 105 against 8).
+MAX_DECODE_ROWS = 96
 
 _GROUP = 32
 

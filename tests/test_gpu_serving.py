@@ -409,6 +409,23 @@ def test_a_cache_takes_the_general_route_too():
         assert (out.double() - ref).norm() <= 2e-2 * ref.norm()
 
 
+@pytest.mark.parametrize("Hq,H,T,D,lens,page", [(12, 1, 8, 128, [300, 0, 5000], 64), (13, 1, 5, 64, [1, 700], 48),
+                                                (56, 4, 6, 128, [2500] * 9, 64), (52, 1, 2, 128, [260, 90], 32)])
+def test_many_rows(Hq, H, T, D, lens, page):
+    """65 to 96 rows a KV head in place, 104 through the unpacked prefix (k and v rounded to bf16 there)."""
+    from maskahead_b200.serving import MAX_DECODE_ROWS
+
+    B = len(lens)
+    cache = _make(B, H, D, lens, page, seed=50)
+    q, kc, vc = _inputs(B, Hq, H, T, D, T, seed=51)
+    out = cache.attend(q, kc, vc)
+    ref, tol = _attend_ref(q, cache.prefix(), kc, vc)
+    if Hq // H * T <= MAX_DECODE_ROWS:
+        _close(out, ref, tol)
+    else:
+        assert (out.double() - ref).norm() <= 2e-2 * ref.norm()
+
+
 def test_a_capture_needs_the_workspace_first(monkeypatch):
     import maskahead_b200.serving as serving
 
