@@ -189,27 +189,34 @@ __device__ __forceinline__ void store_row4(const DecodeParams& p, int b, int h, 
   store4(dst, o.x, o.y, o.z, o.w);
 }
 
-// A CTA's result from nsrc sources in shared memory -- sRows[nsrc][ROWS][kPad] unnormalized
-// rows, sML[nsrc][ROWS] their (m, l) -- to the output rows (normalized) or to partial `slot`.
+// A CTA's result from its sources in shared memory -- the block's keys (source 0, unless `skip`) and
+// the warps: sRows[1 + W][ROWS][kPad] unnormalized rows, sML[1 + W][ROWS] their (m, l) -- to the
+// output rows (normalized) or to partial `slot`. A short sequence leaves most warps without a tile, whose rows
+// are not read.
 template <int D, int ROWS, int W>
-__device__ __forceinline__ void combine(const DecodeParams& p, int b, int h, int r0, int rows, int nsrc, const float* sRows,
+__device__ __forceinline__ void combine(const DecodeParams& p, int b, int h, int r0, int rows, int skip, const float* sRows,
                                         const float2* sML, float2* ml, float* acc) {
   constexpr int kVec = D / 4, kPad = D + 4;
 #pragma unroll 1
   for (int i = threadIdx.x; i < rows * kVec; i += W * 32) {
     const int r = i / kVec, d = (i % kVec) * 4;
+    float2 e[W + 1];
     float m = -INFINITY;
-#pragma unroll 3
-    for (int w = 0; w < nsrc; ++w) m = fmaxf(m, sML[w * ROWS + r].x);
+#pragma unroll
+    for (int w = 0; w <= W; ++w) {
+      e[w] = sML[w * ROWS + r];
+      if (w == 0 && skip) e[w] = make_float2(-INFINITY, 0.f);
+      m = fmaxf(m, e[w].x);
+    }
     const float ms = m == -INFINITY ? 0.f : m;
     float l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 3
-    for (int w = 0; w < nsrc; ++w) {
-      const float2 e = sML[w * ROWS + r];
-      const float f = ex2(e.x - ms);
+#pragma unroll
+    for (int w = 0; w <= W; ++w) {
+      const float f = ex2(e[w].x - ms);
+      if (f == 0.f) continue;          // (a NaN counts)
       const float4 v = *reinterpret_cast<const float4*>(sRows + (w * ROWS + r) * kPad + d);
-      l = fmaf(f, e.y, l);
+      l = fmaf(f, e[w].y, l);
       o.x = fmaf(f, v.x, o.x);
       o.y = fmaf(f, v.y, o.y);
       o.z = fmaf(f, v.z, o.z);
@@ -293,7 +300,7 @@ __device__ __forceinline__ void merge_partials(const DecodeParams& p, const Segm
 // The CTA's rows: the output when they are the sequence's only split, else this split's partial
 // and, in the last CTA to arrive, the merge of all of them.
 template <int D, int ROWS, int W>
-__device__ __forceinline__ void finish(const DecodeParams& p, const Segment& s, int h, int rt, int share, int nsrc,
+__device__ __forceinline__ void finish(const DecodeParams& p, const Segment& s, int h, int rt, int share, int skip,
                                        const float* sRows, const float2* sML, char* buf, int cap) {
   __shared__ int sLast;
   const int r0 = rt * ROWS, rows = min(ROWS, p.R - r0);
@@ -303,7 +310,7 @@ __device__ __forceinline__ void finish(const DecodeParams& p, const Segment& s, 
   float* acc = p.acc + base * D;
   const int64_t slot = partial_slot(s.first, share) * (int64_t)ROWS;
   const bool whole = s.count == 1;
-  combine<D, ROWS, W>(p, b, h, r0, rows, nsrc, sRows, sML, ml + slot, whole ? nullptr : acc + slot * D);
+  combine<D, ROWS, W>(p, b, h, r0, rows, skip, sRows, sML, ml + slot, whole ? nullptr : acc + slot * D);
   if (whole) return;
   __threadfence();
   __syncthreads();
@@ -1048,8 +1055,7 @@ __global__ void __launch_bounds__(W * 32, MINB) decode_attention_kernel(const __
     }
     __syncthreads();
     const int skip = with_block ? 0 : 1;
-    finish<D, ROWS, W>(p, seg, h, rt, (int)blockIdx.x - seg.first, W + 1 - skip, sRows + skip * ROWS * kPad, sML + skip * ROWS,
-                        smem, (int)(decode_smem<D, NT, W>() / (ROWS * (D * 4 + 8))));
+    finish<D, ROWS, W>(p, seg, h, rt, (int)blockIdx.x - seg.first, skip, sRows, sML, smem, (int)(decode_smem<D, NT, W>() / (ROWS * (D * 4 + 8))));
     if (seg.next_unit >= stop) return;
     const int nb = seg.b + 1, at = seg.next_unit, start = seg.next_start;
     __syncthreads();                 // the rows lie over the next sequence's rings
