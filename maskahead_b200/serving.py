@@ -81,8 +81,19 @@ def _check(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple, device:
                          f"got {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
+class _FixedTensors:
+    """The kernels are given the addresses of these objects' tensors once: a tensor is written
+    into, not replaced."""
+
+    def __setattr__(self, name: str, value) -> None:
+        held = self.__dict__.get(name)
+        if isinstance(held, torch.Tensor) and value is not held:
+            raise AttributeError(f"{type(self).__name__}.{name} is fixed for the object's life: write into the tensor")
+        super().__setattr__(name, value)
+
+
 # --------------------------------------------------------------------------- slot planning
-class TokenPlan:
+class TokenPlan(_FixedTensors):
     """The slots of a step's new tokens, planned on the device from the requests' lengths.
 
     lens [B] int32 and pages [B, width] int32 describe the requests now (request b holds
@@ -148,14 +159,14 @@ class TokenPlan:
 
 
 # ----------------------------------------------------------------------------- the cache
-class PagedCache:
+class PagedCache(_FixedTensors):
     """A pool of token-mode k4v4 pages with its requests' tables.
 
     kq, vq [P, H, page_size, D/32, 16] uint8 codes, ks, kz, vs, vz [P, H, page_size, D/32]
     float16, kchan [B, H, D] float32 key divisors, pages [B, max_pages] int32, lens [B]
     int32; free [P] int32 and free_count [1] int32 (optional) the stack of unused pages. The
-    cache addresses these tensors for its life; lens and pages are read on the device by
-    every call.
+    cache addresses these tensors for its life (they are written into, not replaced); lens and
+    pages are read on the device by every call.
     """
 
     def __init__(self, *, kq, ks, kz, vq, vs, vz, kchan, pages, lens, free=None, free_count=None):

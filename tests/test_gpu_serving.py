@@ -318,6 +318,22 @@ def test_strides_and_out():
     assert torch.equal(cache.attend(odd, kc, vc), want)
 
 
+def test_tensors_are_written_into_not_replaced():
+    """The calls keep the tensors' addresses: a new tensor in their place would not be read."""
+    cache = _make(1, 1, 64, [10], 16, seed=60)
+    plan = cache.plan(max_tokens=4) if cache.free is not None else None
+    for name in ("kq", "lens", "pages", "kchan"):
+        with pytest.raises(AttributeError):
+            setattr(cache, name, getattr(cache, name).clone())
+    q, _, _ = _inputs(1, 1, 1, 1, 64, 0, seed=60)
+    before = cache.attend(q)
+    cache.lens.fill_(3)
+    assert not torch.equal(cache.attend(q), before)
+    if plan is not None:
+        with pytest.raises(AttributeError):
+            plan.slots = plan.slots.clone()
+
+
 def test_sliced_pool():
     """A layer's slice of a stacked pool: the page stride is not the page's size."""
     from maskahead_b200.serving import PagedCache
