@@ -84,11 +84,12 @@ class MaPagePlan(ctypes.Structure):
 
 # Argument structs of calls made once a token: packed by struct.Struct, which takes a tenth of the
 # time of filling a ctypes structure (2 us a call). Native alignment; the fields in the header's
-# order, ma_decode_args split into what changes from call to call and what a form of call keeps.
+# order, two of them split into what changes from call to call and what a form of call keeps.
 APPEND_ARGS = struct.Struct("@6P4q2iP4i")          # ma_append_args
 DECODE_HEAD = struct.Struct("@5PN")                # ma_decode_args: q, k, v, out, workspace, workspace_bytes
 DECODE_TAIL = struct.Struct("@12qP8ifi")           # ... sq, sk, sv, so, kv, dtype .. causal, scale, reserved
-VERIFY_ARGS = struct.Struct("@8PN4q4i")            # ma_verify_args
+VERIFY_HEAD = struct.Struct("@8PN")                # ma_verify_args: target .. workspace, workspace_bytes
+VERIFY_TAIL = struct.Struct("@4q4i")               # ... st, sd, dtype, B, K, V
 
 _P = ctypes.POINTER
 _vp, _i32, _f32, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_size_t

@@ -22,12 +22,11 @@ tensor of decode_workspace_bytes / verify_workspace_bytes / PLAN_WORKSPACE_BYTES
 from __future__ import annotations
 
 import ctypes
-import functools
 
 import torch
 
 from . import _lib
-from ._lib import APPEND_ARGS, DECODE_HEAD, DECODE_TAIL, VERIFY_ARGS
+from ._lib import APPEND_ARGS, DECODE_HEAD, DECODE_TAIL, VERIFY_HEAD, VERIFY_TAIL
 from .layouts import Prefix, as_prefix, kv_descriptor
 
 __all__ = ["PagedCache", "TokenPlan", "decode_attention", "verify_drafts", "decode_workspace_bytes",
@@ -70,7 +69,6 @@ def decode_workspace_bytes(batch: int, heads: int, rows: int, head_dim: int, blo
     return int(_lib.load_library().ma_decode_attention_workspace(batch, heads, rows, head_dim, block_tokens))
 
 
-@functools.lru_cache(maxsize=256)
 def verify_workspace_bytes(batch: int, vocab: int) -> int:
     return int(_lib.load_library().ma_verify_drafts_workspace(batch, vocab))
 
@@ -442,6 +440,35 @@ def verify_drafts(target: torch.Tensor, draft: torch.Tensor | None, tokens: torc
     Returns (accepted [B] int32, tokens [B, K + 1] int32: the accepted drafts, the next token,
     then -1); tokens[b, accepted[b]] is -1 only when p_a has no mass.
     """
+    form = (target.shape, target.stride(), target.dtype, target.get_device(), tokens.shape, tokens.stride(), tokens.dtype,
+            tokens.get_device(), uniforms.shape, uniforms.stride(), uniforms.dtype, uniforms.get_device(),
+            None if draft is None else (draft.shape, draft.stride(), draft.dtype, draft.get_device()),
+            None if counts is None else (counts.shape, counts.stride(), counts.dtype, counts.get_device()))
+    tail = _verify_forms.get(form)
+    if tail is None:
+        tail = _verify_form(target, draft, tokens, counts, uniforms)
+        if len(_verify_forms) >= _MAX_FORMS:
+            _verify_forms.clear()
+        _verify_forms[form] = tail
+    accepted = uniforms.new_empty(tail[0], dtype=torch.int32) if counts is None else torch.empty_like(counts)
+    out = torch.empty_like(uniforms, dtype=torch.int32)
+    dev = target.device
+    ws, nbytes = _scratch(dev, "verify", tail[1], workspace)
+    rc = _lib.lib().ma_verify_drafts(VERIFY_HEAD.pack(
+        target.data_ptr(), 0 if draft is None else draft.data_ptr(), tokens.data_ptr(),
+        0 if counts is None else counts.data_ptr(), uniforms.data_ptr(), accepted.data_ptr(), out.data_ptr(), ws, nbytes)
+        + tail[2], _lib.stream_handle(dev))
+    if rc:
+        _lib.check("ma_verify_drafts", rc)
+    return accepted, out
+
+
+# Forms of call (shapes, strides, types, devices) that passed the checks: (requests, workspace bytes, the
+# packed end of ma_verify_args). The checks took a third of a small call's host time.
+_verify_forms: dict[tuple, tuple[int, int, bytes]] = {}
+
+
+def _verify_form(target, draft, tokens, counts, uniforms) -> tuple[int, int, bytes]:
     shape, index = target.shape, target.get_device()
     b, k1, v = shape if len(shape) == 3 else (0, 0, 0)
     k = k1 - 1
@@ -455,18 +482,8 @@ def verify_drafts(target: torch.Tensor, draft: torch.Tensor | None, tokens: torc
             or (draft is not None and (draft.dtype is not target.dtype or draft.shape != (b, k, v)
                                        or draft.get_device() != index or (draft.stride(2) != 1 and v > 1)))):
         _refuse_verify(target, draft, tokens, counts, uniforms)
-    dev = target.device
-    accepted = uniforms.new_empty(b, dtype=torch.int32) if counts is None else torch.empty_like(counts)
-    out = tokens.new_empty((b, k1))
-    ws, nbytes = _scratch(dev, "verify", verify_workspace_bytes(b, v), workspace)
     st, sd = target.stride(), (0, 0) if draft is None else draft.stride()
-    rc = _lib.lib().ma_verify_drafts(VERIFY_ARGS.pack(
-        target.data_ptr(), 0 if draft is None else draft.data_ptr(), tokens.data_ptr(),
-        0 if counts is None else counts.data_ptr(), uniforms.data_ptr(), accepted.data_ptr(), out.data_ptr(), ws, nbytes,
-        st[0], st[1], sd[0], sd[1], code, b, k, v), _lib.stream_handle(dev))
-    if rc:
-        _lib.check("ma_verify_drafts", rc)
-    return accepted, out
+    return b, verify_workspace_bytes(b, v), VERIFY_TAIL.pack(st[0], st[1], sd[0], sd[1], code, b, k, v)
 
 
 _PROBABILITIES = {torch.float32: _lib.MA_F32, torch.bfloat16: _lib.MA_BF16, torch.float16: _lib.MA_F16}

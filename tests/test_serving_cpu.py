@@ -25,9 +25,9 @@ def _append(pool=None, k=0, n=1, dtype=1, d=128):
 
 
 def _verify(target=16, vocab=8, dtype=0, ws=0, nbytes=0):
-    from maskahead_b200._lib import VERIFY_ARGS
+    from maskahead_b200._lib import VERIFY_HEAD, VERIFY_TAIL
 
-    return VERIFY_ARGS.pack(target, 16, 16, 0, 16, 16, 16, ws, nbytes, 0, 0, 0, 0, dtype, 1, 1, vocab)
+    return VERIFY_HEAD.pack(target, 16, 16, 0, 16, 16, 16, ws, nbytes) + VERIFY_TAIL.pack(0, 0, 0, 0, dtype, 1, 1, vocab)
 
 
 def test_rejected_arguments(lib):
@@ -60,7 +60,7 @@ def test_packed_structs_match_the_header(tmp_path):
     import subprocess
     from pathlib import Path
 
-    from maskahead_b200._lib import APPEND_ARGS, DECODE_HEAD, DECODE_TAIL, VERIFY_ARGS
+    from maskahead_b200._lib import APPEND_ARGS, DECODE_HEAD, DECODE_TAIL, VERIFY_HEAD, VERIFY_TAIL
 
     cc = shutil.which("gcc") or shutil.which("cc")
     if cc is None:
@@ -74,7 +74,7 @@ def test_packed_structs_match_the_header(tmp_path):
     subprocess.run([cc, "-I", str(root / "include"), str(src), "-o", str(exe)], check=True)
     got = [int(x) for x in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()]
     head, tail = DECODE_HEAD.size, DECODE_TAIL.size
-    assert got == [APPEND_ARGS.size, 88, head + tail, head, head + 12 * 8 + 8 + 8 * 4, VERIFY_ARGS.size, 72]
+    assert got == [APPEND_ARGS.size, 88, head + tail, head, head + 12 * 8 + 8 + 8 * 4, VERIFY_HEAD.size + VERIFY_TAIL.size, VERIFY_HEAD.size]
 
 
 def test_page_plan_struct_matches_the_header(lib):
