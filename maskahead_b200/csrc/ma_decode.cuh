@@ -1055,7 +1055,8 @@ __global__ void __launch_bounds__(W * 32, MINB) decode_attention_kernel(const __
     }
     __syncthreads();
     const int skip = with_block ? 0 : 1;
-    finish<D, ROWS, W>(p, seg, h, rt, (int)blockIdx.x - seg.first, skip, sRows, sML, smem, (int)(decode_smem<D, NT, W>() / (ROWS * (D * 4 + 8))));
+    finish<D, ROWS, W>(p, seg, h, rt, (int)blockIdx.x - seg.first, skip, sRows, sML, smem,
+                       (int)(decode_smem<D, NT, W>() / (ROWS * (D * 4 + 8))));
     if (seg.next_unit >= stop) return;
     const int nb = seg.b + 1, at = seg.next_unit, start = seg.next_start;
     __syncthreads();                 // the rows lie over the next sequence's rings
