@@ -247,6 +247,29 @@ def test_masks(paged):
             assert torch.count_nonzero(out[0, 2:4]) == 0
 
 
+@pytest.mark.parametrize("B,Hq,H,D,T", [(2, 14, 2, 128, 3), (400, 3, 1, 64, 1)])
+def test_a_cache_without_slots_needs_no_arrays(B, Hq, H, D, T):
+    """nq = 0 and null pointers, as the other C entries take an empty cache: the block's keys alone.
+    (Both launch forms: few sequences, and more of them than SMs.)"""
+    import ctypes
+
+    from maskahead_b200._lib import DECODE_HEAD, DECODE_TAIL, MA_BF16, MA_KV_PACKED_TOKEN, MaKV, lib
+    from maskahead_b200.serving import decode_workspace_bytes
+
+    q, kc, vc = _inputs(B, Hq, H, T, D, T, seed=61)
+    kv = MaKV()
+    kv.layout, kv.dtype = MA_KV_PACKED_TOKEN, MA_BF16
+    out = torch.empty_like(q)
+    ws = torch.zeros(decode_workspace_bytes(B, H, Hq // H * T, D, T), dtype=torch.uint8, device=DEV)
+    rc = lib().ma_decode_attention(
+        DECODE_HEAD.pack(q.data_ptr(), kc.data_ptr(), vc.data_ptr(), out.data_ptr(), ws.data_ptr(), ws.numel())
+        + DECODE_TAIL.pack(*q.stride()[:3], *kc.stride()[:3], *vc.stride()[:3], *out.stride()[:3], ctypes.addressof(kv),
+                           MA_BF16, B, Hq, H, T, D, T, 1, D ** -0.5, 0), torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    # the same requests in a cache whose lengths are 0
+    assert torch.equal(out, _make(B, H, D, [0] * B, 32, seed=62).attend(q, kc, vc))
+
+
 def test_bad_pages_read_as_dead():
     cache = _make(2, 2, 128, [200, 200], 32, seed=10)
     cache.pages[0, 1] = -1
