@@ -282,10 +282,18 @@ __global__ void __launch_bounds__(kThreads) page_plan_kernel(const __grid_consta
 int page_plan_max_requests() { return kMaxRequests; }
 
 int launch_page_plan(PagePlanParams& p, cudaStream_t st) {
+  // what the largest call takes is opted in to once per device: the default limit of 48 KB holds for
+  // the dynamic bytes and the kernel's static ones together
+  constexpr size_t kMost = (5 * (size_t)kMaxRequests + 3) * sizeof(int);
+  static bool ready[64] = {false};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return MA_ERR_CUDA;
+  if (dev < 0 || dev >= 64 || !ready[dev]) {
+    if (cudaFuncSetAttribute(page_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMost) != cudaSuccess)
+      return MA_ERR_CUDA;
+    if (dev >= 0 && dev < 64) ready[dev] = true;
+  }
   const size_t smem = (5 * (size_t)p.B + 3) * sizeof(int);
-  if (smem > 48 * 1024 &&
-      cudaFuncSetAttribute(page_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-    return MA_ERR_CUDA;
   int64_t items = ((int64_t)p.max_tokens + 3) / 4;
   if (!p.pages_in_place) items = items > (int64_t)p.B * p.width ? items : (int64_t)p.B * p.width;
   if (!p.free_in_place) items = items > p.num_pages ? items : p.num_pages;

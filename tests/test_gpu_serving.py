@@ -705,6 +705,29 @@ def test_page_plan_many_requests_and_refusals():
         many.build(i32(8193))
 
 
+def test_page_plan_around_the_default_shared_memory_limit():
+    """Request counts whose arrays end just below 48 KB, the kernel's static bytes above it, in a process
+    that has planned nothing larger."""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    code = """
+import torch
+from maskahead_b200.serving import TokenPlan
+i32 = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")
+for B in (2446, 2447, 2452, 2457, 2458):
+    plan = TokenPlan(lens=i32(B), pages=i32(B, 1), free=torch.arange(B, dtype=torch.int32, device="cuda"),
+                     free_count=i32(1) + B, page_size=16, num_pages=B, max_tokens=B)
+    plan.build(i32(B) + 1)
+    assert plan.lens.eq(1).all() and int(plan.free_count) == 0 and plan.seqs.tolist() == list(range(B))
+    assert sorted(plan.slots.tolist()) == [16 * p for p in range(B)]
+"""
+    root = Path(__file__).resolve().parents[1]
+    done = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
+
+
 # ------------------------------------------------------------------------------ append
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("N,H,D,page", [(1, 1, 128, 16), (5, 3, 64, 7), (33, 4, 128, 64), (300, 2, 128, 48), (4097, 1, 64, 32)])
