@@ -747,6 +747,18 @@ __device__ __forceinline__ void attn_fa_body(const Args& A) {
         tmem_st_wait();
         l_run += (acc0.x + acc0.y) + (acc1.x + acc1.y);
       }
+      // a ragged batch: what the cache holds past lens[b] is not the sequence's, and 0 * NaN is NaN, so
+      // those rows of its last V tile become zeros before P V reads them, a row per warp of the group
+      // at a time (PAIR: both groups write the same zeros)
+      const int exist = end - (begin + t * kBN);
+      if (!dq && !is_cur && A.kv.lens && t < ntp && exist < kBN) {
+        if (!mbar_wait(&vfull[t % VS], (uint32_t)(t / VS) & 1u)) s_abort = 1;
+        uint32_t dead = smem_addr(sVs + (t % VS) * kKVBytes + (lane >> 4) * kKVBlock + (lane & 15) * 8) + (exist + quarter) * 128;
+#pragma unroll 1
+        for (int row = exist + quarter; row < kBN; row += 4, dead += 512)
+          asm volatile("st.shared.v2.u32 [%0], {%1, %1};\n" ::"r"(dead), "r"(0u) : "memory");
+        fence_proxy_async();   // generic stores -> the tensor core's reads
+      }
       fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[grp]);

@@ -465,6 +465,46 @@ def test_many_rows(Hq, H, T, D, lens, page):
         assert (out.double() - ref).norm() <= 2e-2 * ref.norm()
 
 
+@pytest.mark.parametrize("Hq,H,T,lens,page", [(13, 1, 8, [300, 0, 5000], 64), (56, 4, 8, [2500] * 3, 64), (104, 2, 2, [260, 90], 32)])
+def test_general_route_scratch_past_the_lengths(Hq, H, T, lens, page):
+    """What an earlier call left in the unpacked copy behind the lengths, NaN included, is not read."""
+    from maskahead_b200 import _lib
+
+    B = len(lens)
+    cache = _make(B, H, 128, lens, page, seed=63)
+    q, kc, vc = _inputs(B, Hq, H, T, 128, T, seed=64)
+    cache.attend(q, kc, vc)
+    for purpose in ("unpack_k", "unpack_v"):
+        _lib.workspace(q.device, purpose, 1).fill_(0xFF)          # bf16 NaN
+    out = cache.attend(q, kc, vc)
+    ref, _ = _attend_ref(q, cache.prefix(), kc, vc)
+    assert torch.isfinite(out).all()
+    assert (out.double() - ref).norm() <= 2e-2 * ref.norm()       # as test_many_rows
+
+
+@pytest.mark.parametrize("Hq,T", [(28, 1), (28, 32), (8, 32)])
+def test_dense_ragged_caches_hold_anything_past_the_lengths(Hq, T):
+    from maskahead_b200.layouts import Prefix
+    from maskahead_b200.serving import decode_attention
+
+    B, H, n, D = 3, 4, 700, 128
+    g = torch.Generator().manual_seed(65)
+    k = torch.randn(B, H, n, D, generator=g).to(torch.bfloat16).to(DEV)
+    v = torch.randn(B, H, n, D, generator=g).to(torch.bfloat16).to(DEV)
+    q, kc, vc = _inputs(B, Hq, H, T, D, T, seed=66)
+    lens = torch.tensor([238, 17, 697], dtype=torch.int32, device=DEV)
+    outs = []
+    for rest in (0.0, float("nan"), float("inf")):
+        for b in range(B):
+            k[b, :, int(lens[b]):] = rest
+            v[b, :, int(lens[b]):] = rest
+        pre = Prefix.dense(k, v)
+        pre.lens = lens
+        outs.append(decode_attention(q, pre, kc, vc))
+    assert torch.isfinite(outs[0]).all()
+    assert torch.equal(outs[1], outs[0]) and torch.equal(outs[2], outs[0])
+
+
 def test_a_capture_needs_the_workspace_first(monkeypatch):
     import maskahead_b200.serving as serving
 
