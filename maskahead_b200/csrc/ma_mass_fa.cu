@@ -299,9 +299,7 @@ __device__ __forceinline__ void mass_fa_body(const Args& A) {
         if (!ok || s_abort) break;
         const uint8_t* sV = sSlot + (nK + t % nV) * kTileBytes;
         const float* a = sA[t & 1];
-#pragma unroll 8
-        for (int i = 0; i < 64; ++i) {
-          const int j = 64 * cw + i;
+        auto add = [&](int j) {
           const float aj = a[j];
           const uint2 u = *reinterpret_cast<const uint2*>(sV + chunk_off(j, lane >> 1) + lane_off);
           const float2 v0 = make_float2(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xFFFF0000u));
@@ -309,6 +307,17 @@ __device__ __forceinline__ void mass_fa_body(const Args& A) {
           cacc0 = ffma2(make_float2(aj, aj), v0, cacc0);
           cacc1 = ffma2(make_float2(aj, aj), v1, cacc1);
           asum += aj;
+        };
+        // a dead slot (a_j = 0: masked, or past a ragged batch's lens[b]) holds whatever the cache
+        // does, and 0 * NaN is NaN
+        const int first = 64 * cw, exist = end - (begin + t * kTile) - first;
+        if (exist >= 64 && A.kv.mask == nullptr) {
+#pragma unroll 8
+          for (int i = 0; i < 64; ++i) add(first + i);
+        } else {
+#pragma unroll 4
+          for (int i = 0; i < 64; ++i)
+            if (a[first + i] != 0.f) add(first + i);
         }
         __syncwarp();
         if (lane == 0) {

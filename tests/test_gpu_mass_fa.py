@@ -160,3 +160,32 @@ def test_mass_fa_ragged_batch_split_matches_oracle(B, n, cap):
         assert not mass[bi, :, L:].any() and not score[bi, :, L:].any(), "slots past the length must be 0"
     np.testing.assert_allclose(mass.numpy(), out[-1][0].numpy(), rtol=2e-5, atol=1e-9)
     np.testing.assert_allclose(score.numpy(), out[-1][1].numpy(), rtol=5e-5, atol=1e-9)
+
+
+@pytest.mark.parametrize("kind", ["lens", "mask"])
+def test_dead_slots_may_hold_anything(kind):
+    """NaN and infinities in slots past the lengths, or masked out, leave every score as it is."""
+    from maskahead_b200.kernels import prefix_scores, splitk_attention
+    from maskahead_b200.layouts import Prefix
+
+    gen = torch.Generator().manual_seed(77)
+    B, Hq, H, T, n, D = 3, 8, 2, 32, 700, 128
+    q = torch.randn(B, Hq, T, D, generator=gen).to(torch.bfloat16).to(DEV)
+    k = torch.randn(B, H, n, D, generator=gen).to(torch.bfloat16).to(DEV)
+    v = torch.randn(B, H, n, D, generator=gen).to(torch.bfloat16).to(DEV)
+    lens = torch.tensor([238, 17, 697], dtype=torch.int32)
+    if kind == "lens":
+        live = (torch.arange(n)[None] < lens[:, None])[:, None].expand(B, H, n).to(DEV)
+        extra = dict(lens=lens.to(DEV))
+    else:
+        live = (torch.rand(B, H, n, generator=gen) > 0.3).to(DEV)
+        extra = dict(mask=live)
+    outs = []
+    for rest in (0.0, float("nan"), float("inf")):
+        k[~live], v[~live] = rest, rest
+        pre = Prefix(kf=k, vf=v, nf=n, **extra)
+        _, st = splitk_attention(q, pre, None, None, want_prefix=True)
+        outs.append(prefix_scores(q, pre, st, list(range(T)), value=True))
+    assert all(torch.isfinite(x).all() for x in outs[0]) and not outs[0][1][~live].any()
+    for mass, score in outs[1:]:
+        assert torch.equal(mass, outs[0][0]) and torch.equal(score, outs[0][1])
