@@ -25,7 +25,7 @@ __all__ = ["Prefix", "splitk_attention", "prefix_scores", "dequantize_prefix"]
 
 def splitk_attention(query, prefix, current_key, current_value, *, scaling=None,
                      causal_block: int = 0, q_pos0: int = 0, c_pos0: int = 0, want_prefix: bool = False,
-                     stats_out=None, head_gather=None, **_tuning):
+                     stats_out=None, head_gather=None, workspace: torch.Tensor | None = None, **_tuning):
     """softmax over [prefix | current] for every query row (splitk.py:493-579).
 
     Returns (out [B,Hq,T,D] in the query dtype, stats) with stats = (M_p, L_p, O_p,
@@ -40,6 +40,8 @@ def splitk_attention(query, prefix, current_key, current_value, *, scaling=None,
     t < gathered.shape[2] are exchanged with every rank's in the same launch (the split
     merge stores them into every rank's receive region) and gathered holds all of them,
     [B, world * Hq, Tg, D] bf16, when the call returns on the stream.
+    workspace: scratch of the caller's (uint8, at least ma_prefix_attention_workspace bytes, its
+    error word and counters zero) instead of the device's shared one.
     """
     lib = _lib.lib()
     prefix = as_prefix(prefix)
@@ -75,7 +77,7 @@ def splitk_attention(query, prefix, current_key, current_value, *, scaling=None,
     else:
         mp = lp = op = None
     nbytes = lib.ma_prefix_attention_workspace(b, hkv, r, prefix.n, d, cur.Tc)
-    ws = _lib.workspace(dev, "attention", nbytes)
+    ws = workspace if workspace is not None else _lib.workspace(dev, "attention", nbytes)
     scale = float(scaling if scaling is not None else d ** -0.5)
     if head_gather is not None:
         gather, gout = head_gather

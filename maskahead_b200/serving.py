@@ -16,7 +16,8 @@ first axis. Everything runs on the current stream of the pool's device without w
 it, and can be captured in a CUDA graph (run once before the capture, so that the shared
 workspace exists). Calls share one workspace per device and purpose, like the other
 operators: calls that can overlap on the GPU pass their own (`workspace`, a zeroed uint8
-tensor of decode_workspace_bytes / verify_workspace_bytes / PLAN_WORKSPACE_BYTES).
+tensor of decode_workspace_bytes / verify_workspace_bytes / PLAN_WORKSPACE_BYTES; attention
+that is not read in place needs decode_workspace_bytes with its `capacity`).
 """
 
 from __future__ import annotations
@@ -64,9 +65,31 @@ def _scratch(device: torch.device, purpose: str, nbytes: int, given: torch.Tenso
     return given.data_ptr(), given.numel()
 
 
-def decode_workspace_bytes(batch: int, heads: int, rows: int, head_dim: int, block_tokens: int = 0) -> int:
-    """Workspace of decode_attention: rows = query heads per KV head x tokens."""
-    return int(_lib.load_library().ma_decode_attention_workspace(batch, heads, rows, head_dim, block_tokens))
+def decode_workspace_bytes(batch: int, heads: int, rows: int, head_dim: int, block_tokens: int = 0, *,
+                           capacity: int = 0) -> int:
+    """Workspace of decode_attention: rows = query heads per KV head x tokens. With capacity =
+    the prefix's slots per sequence (max_pages * page_size of a paged cache), also of calls that
+    are not read in place: those keep the unpacked prefix and splitk_attention's scratch in it
+    (device_status looks at the shared workspaces only: a wait that gave up in a caller's shows as
+    rows of NaN)."""
+    nbytes = int(_lib.load_library().ma_decode_attention_workspace(batch, heads, rows, head_dim, block_tokens))
+    if nbytes == 0 or capacity <= 0:
+        return nbytes
+    return _general_layout(batch, heads, rows, head_dim, block_tokens, capacity, True)[2]
+
+
+# splitk_attention's error word and merge counters lie in the first bytes of its scratch
+_SPLITK_HEAD = 1 << 17
+
+
+def _general_layout(batch, heads, rows, head_dim, block_tokens, slots, unpack) -> tuple[int, int, int]:
+    """A caller's workspace on the general route: (offset and bytes of splitk_attention's scratch, end),
+    from its first 256-byte boundary, the unpacked K and V behind the scratch. All of it lies behind
+    what an in-place call of these sizes uses, whose counters are zero between calls."""
+    lib, up = _lib.load_library(), lambda x: (x + 255) & ~255  # noqa: E731
+    at = up(int(lib.ma_decode_attention_workspace(batch, heads, rows, head_dim, block_tokens)))
+    scratch = up(int(lib.ma_prefix_attention_workspace(batch, heads, rows, slots, head_dim, block_tokens))) + 256
+    return at, scratch, at + scratch + (2 * up(2 * batch * heads * slots * head_dim) if unpack else 0) + 256
 
 
 def verify_workspace_bytes(batch: int, vocab: int) -> int:
@@ -289,7 +312,8 @@ def decode_attention(query: torch.Tensor, prefix, current_key: torch.Tensor | No
     Token-mode k4v4 storage without a dense tail (contiguous or paged, ragged, masked) is read
     in place when the query is bfloat16 and a KV head has at most MAX_DECODE_ROWS rows; its
     elements are then not rounded to bfloat16. Everything else runs as splitk_attention,
-    over a bfloat16 copy of a packed prefix. A row that sees no key is zero.
+    over a bfloat16 copy of a packed prefix. A row that sees no key is zero. workspace: see
+    decode_workspace_bytes; one too small for the route of the call is refused.
     """
     if isinstance(prefix, PagedCache):
         return _attend(query, prefix, prefix._desc, current_key, current_value, scaling, causal, out, workspace)
@@ -331,7 +355,7 @@ def _attend(query, source, desc, current_key, current_value, scaling, causal, ou
             return _attend(q2, source, desc, k2, v2, scaling, causal, out, workspace)
         call = _attend_form(query, source, desc, current_key, current_value, scaling, causal, out)
         if call is None:
-            return _attend_general(query, source, current_key, current_value, scaling, causal, out)
+            return _attend_general(query, source, current_key, current_value, scaling, causal, out, workspace)
         if forms is not None:
             if len(forms) >= _MAX_FORMS:
                 forms.clear()
@@ -351,7 +375,7 @@ def _attend(query, source, desc, current_key, current_value, scaling, causal, ou
     ws, nbytes = _scratch(dev, "decode", call.nbytes, workspace)
     rc = call.run(DECODE_HEAD.pack(q, k, v, o.data_ptr(), ws, nbytes) + call.tail, _lib.stream_handle(dev))
     if rc == _lib.MA_ERR_UNSUPPORTED:
-        return _attend_general(query, source, current_key, current_value, scaling, causal, out)
+        return _attend_general(query, source, current_key, current_value, scaling, causal, out, workspace)
     if rc:
         _lib.check("ma_decode_attention", rc)
     return o
@@ -406,17 +430,31 @@ def _attend_form(query, source, desc, current_key, current_value, scaling, causa
     return call
 
 
-def _attend_general(query, source, current_key, current_value, scaling, causal, out):
+def _attend_general(query, source, current_key, current_value, scaling, causal, out, workspace):
     from .hotpath import unpacked_prefix
     from .kernels.splitk import splitk_attention
 
     prefix = source.prefix() if isinstance(source, PagedCache) else source
     b, hq, t, d = query.shape
-    if query.dtype == torch.bfloat16 and prefix.nq > 0:
-        prefix = unpacked_prefix(prefix, b, prefix.vq.shape[1], d)
     tc = 0 if current_key is None else current_key.shape[2]
+    stored = prefix.kf if prefix.kf is not None else prefix.vq
+    heads = stored.shape[1] if current_key is None else current_key.shape[1]
+    unpack = query.dtype == torch.bfloat16 and prefix.nq > 0
+    scratch = unpacked = None
+    if workspace is not None:      # nothing shared: the call's scratch and copies lie in what it was given
+        at, nbytes, end = _general_layout(b, heads, hq // heads * t, d, tc, prefix.n, unpack)
+        base = -_scratch(query.device, "decode", end, workspace)[0] % 256 + at
+        scratch = workspace[base:base + nbytes]
+        scratch[:_SPLITK_HEAD].zero_()       # (in-place calls leave partials here)
+        if unpack:
+            size, shape = 2 * b * heads * prefix.n * d, (b, heads, prefix.n, d)
+            at_k = base + nbytes
+            at_v = at_k + ((size + 255) & ~255)
+            unpacked = tuple(workspace[x:x + size].view(torch.bfloat16).view(shape) for x in (at_k, at_v))
+    if unpack:
+        prefix = unpacked_prefix(prefix, b, heads, d, out=unpacked)
     res, _ = splitk_attention(query, prefix, current_key, current_value, scaling=scaling,
-                              causal_block=1 if causal and tc else 0, q_pos0=tc - t, c_pos0=0)
+                              causal_block=1 if causal and tc else 0, q_pos0=tc - t, c_pos0=0, workspace=scratch)
     if out is None:
         return res
     out.copy_(res)

@@ -540,6 +540,62 @@ def test_streams_graphs_and_own_workspace():
     assert not torch.equal(out, want)
 
 
+@pytest.mark.parametrize("kind", ["rows", "float32", "channel"])
+def test_general_route_stays_in_its_own_workspace(kind):
+    """With a workspace given, the route through splitk_attention touches no shared scratch, so calls on
+    two streams do not meet; too small a workspace is refused."""
+    from maskahead_b200 import _lib
+    from maskahead_b200.layouts import pack_prefix
+    from maskahead_b200.serving import decode_attention, decode_workspace_bytes
+
+    B, H, D, T, n = 2, 2, 128, 2, 576
+    Hq = 104 if kind == "rows" else 8
+    dtype = torch.float32 if kind == "float32" else torch.bfloat16
+    sources, inputs = [], []
+    for seed in (70, 71):
+        if kind == "channel":
+            g = torch.Generator().manual_seed(seed)
+            k, v = (torch.randn(B, H, n, D, generator=g).to(torch.bfloat16).to(DEV) for _ in range(2))
+            sources.append(pack_prefix(k, v, key_mode="channel"))
+        else:
+            sources.append(_make(B, H, D, [n, 90], 32, seed=seed))
+        inputs.append([x.to(dtype) for x in _inputs(B, Hq, H, T, D, T, seed=seed)])
+    want = [decode_attention(q, s, k, v) for s, (q, k, v) in zip(sources, inputs)]
+    shared = [b for (_, _, purpose), b in _lib._WORKSPACES.items() if purpose in ("attention", "unpack_k", "unpack_v", "decode")]
+    assert shared
+    nbytes = decode_workspace_bytes(B, H, Hq // H * T, D, T, capacity=n)
+    room = [torch.zeros(nbytes + 8, dtype=torch.uint8, device=DEV)[i:nbytes + i] for i in (0, 3)]       # any alignment
+    before = [b.clone() for b in shared]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                q, k, v = inputs[i]
+                got[i].append(decode_attention(q, sources[i], k, v, workspace=room[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(x, want[i]) for x in got[i])
+    assert all(torch.equal(a, b) for a, b in zip(shared, before))
+    with pytest.raises(ValueError):
+        q, k, v = inputs[0]
+        decode_attention(q, sources[0], k, v, workspace=room[0][:1 << 16])
+
+
+def test_one_workspace_serves_both_routes():
+    from maskahead_b200.serving import decode_workspace_bytes
+
+    cache = _make(2, 2, 128, [576, 90], 32, seed=72)
+    few, many = _inputs(2, 14, 2, 2, 128, 2, seed=73), _inputs(2, 104, 2, 2, 128, 2, seed=74)
+    want = [cache.attend(*few), cache.attend(*many)]
+    nbytes = max(decode_workspace_bytes(2, 2, r, 128, 2, capacity=576) for r in (14, 104))
+    ws = torch.zeros(nbytes, dtype=torch.uint8, device=DEV)
+    for _ in range(3):
+        assert torch.equal(cache.attend(*few, workspace=ws), want[0])
+        assert torch.equal(cache.attend(*many, workspace=ws), want[1])
+
+
 def test_attention_refusals():
     import ctypes
 

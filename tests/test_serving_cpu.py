@@ -100,6 +100,18 @@ def test_workspace_sizes(lib):
         assert lib.ma_verify_drafts_workspace(b, v) <= fixed + b * 2048 * 8
 
 
+def test_workspace_of_the_general_route(lib):
+    """It holds an in-place call's part, the split attention's scratch and both unpacked copies."""
+    from maskahead_b200.serving import _SPLITK_HEAD, decode_workspace_bytes
+
+    for b, h, r, d, tc, n in ((1, 1, 1, 64, 0, 1), (2, 2, 104, 128, 2, 576), (32, 4, 224, 128, 32, 8192)):
+        here, split = lib.ma_decode_attention_workspace(b, h, r, d, tc), lib.ma_prefix_attention_workspace(b, h, r, n, d, tc)
+        assert decode_workspace_bytes(b, h, r, d, tc) == here
+        assert decode_workspace_bytes(b, h, r, d, tc, capacity=n) >= here + split + 4 * b * h * n * d
+    # a call of one row and no key: little but the fixed words at the front
+    assert lib.ma_prefix_attention_workspace(1, 1, 1, 0, 128, 0) <= _SPLITK_HEAD
+
+
 @pytest.mark.skipif(torch.cuda.is_available(), reason="checks the no-GPU behaviour")
 def test_no_cpu_path():
     from maskahead_b200 import KernelUnavailableError
