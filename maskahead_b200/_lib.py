@@ -223,7 +223,16 @@ def i64(*vals) -> ctypes.Array:
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
+def current_device() -> int:
+    return torch._C._cuda_getDevice()
+
+
 def stream_handle(device: torch.device) -> int:
+    """The current stream of `device`, for a launch. The library launches on the current device
+    (a default stream's handle says nothing of its device), so `device` has to be that one."""
+    if device.index is not None and device.index != current_device():
+        raise RuntimeError(f"the tensors lie on {device}, but cuda:{current_device()} is the current device: "
+                           f"call within torch.cuda.device({device.index})")
     if _raw_stream is not None and device.index is not None:
         return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
@@ -238,13 +247,7 @@ STATUS_WORKSPACES = frozenset({"attention", "value_score"})
 STATUS_EXTRA: list[tuple[int, torch.Tensor]] = []
 
 
-def device_status(device: torch.device | int | None = None) -> None:
-    """Raise MaError(MA_ERR_TIMEOUT) if a bounded device-side wait of a kernel that used one
-    of this module's workspaces on `device` gave up since the last check (its rows were
-    written as NaN). Waits for the work queued on the device's current stream and clears
-    the recorded errors."""
-    dev = torch.device("cuda", torch.cuda.current_device() if device is None else
-                       (device if isinstance(device, int) else device.index or 0))
+def _failed_waits(dev: torch.device) -> list[str]:
     lib_ = lib()
     stream = stream_handle(dev)
     failed = []
@@ -264,6 +267,19 @@ def device_status(device: torch.device | int | None = None) -> None:
             failed.append("head_gather")
         elif rc != MA_OK:
             check("ma_workspace_status", rc)
+    return failed
+
+
+def device_status(device: torch.device | int | None = None) -> None:
+    """Raise MaError(MA_ERR_TIMEOUT) if a bounded device-side wait of a kernel that used one
+    of this module's workspaces on `device` gave up since the last check (its rows were
+    written as NaN). Waits for the work queued on the device's current stream and clears
+    the recorded errors."""
+    dev = torch.device("cuda", torch.cuda.current_device() if device is None else
+                       (device if isinstance(device, int) else device.index or 0))
+    lib()
+    with torch.cuda.device(dev):
+        failed = _failed_waits(dev)
     if failed:
         detail = load_library().ma_status_string(MA_ERR_TIMEOUT).decode()
         raise MaError("device_status", MA_ERR_TIMEOUT, f"{detail} in the work of: {', '.join(sorted(failed))}")

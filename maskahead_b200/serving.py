@@ -12,8 +12,8 @@ and layer a serving program
 
 The reference has no counterpart (its cache is contiguous, its sessions run one batch);
 the pool's arrays are its token-mode k4v4 layout (cache.py:142-189) with the page as the
-first axis. Everything runs on the current stream of the pool's device without waiting for
-it, and can be captured in a CUDA graph (run once before the capture, so that the shared
+first axis. Everything runs on the current stream of the pool's device (made current for the
+call if another one is) without waiting for it, and can be captured in a CUDA graph (run once before the capture, so that the shared
 workspace exists). Calls share one workspace per device and purpose, like the other
 operators: calls that can overlap on the GPU pass their own (`workspace`, a zeroed uint8
 tensor of decode_workspace_bytes / verify_workspace_bytes / PLAN_WORKSPACE_BYTES; attention
@@ -169,6 +169,9 @@ class TokenPlan(_FixedTensors):
 
     def build(self, new_lens: torch.Tensor, *, workspace: torch.Tensor | None = None) -> "TokenPlan":
         """Plan the step whose requests shall have new_lens [B] int32 tokens; returns self."""
+        if self._index != _lib.current_device():
+            with torch.cuda.device(self._index):
+                return self.build(new_lens, workspace=workspace)
         if (new_lens.dtype is not torch.int32 or new_lens.get_device() != self._index or new_lens.dim() != 1
                 or new_lens.size(0) != self.batch or not new_lens.is_contiguous()):
             _check("new_lens", new_lens, torch.int32, (self.batch,), self.device)
@@ -250,6 +253,9 @@ class PagedCache(_FixedTensors):
         layouts.quantize_tokens. return_rows: also the values the slots now stand for, (k, v)
         [N, H, D] in the rows' type."""
         shape, index, dev = key.shape, self._index, self.device
+        if index != _lib.current_device():
+            with torch.cuda.device(index):
+                return self.append(key, value, slots, seqs, return_rows=return_rows)
         n = shape[0] if len(shape) == 3 else -1
         if (n < 0 or value.shape != shape or value.dtype is not key.dtype or shape[1] != self.heads
                 or shape[2] != self.head_dim or key.get_device() != index or value.get_device() != index
@@ -289,6 +295,10 @@ class PagedCache(_FixedTensors):
                current_value: torch.Tensor | None = None, *, scaling: float | None = None, causal: bool = True,
                out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
         """decode_attention over this cache."""
+        if self._index != _lib.current_device():
+            with torch.cuda.device(self._index):
+                return self.attend(query, current_key, current_value, scaling=scaling, causal=causal, out=out,
+                                   workspace=workspace)
         return _attend(query, self, self._desc, current_key, current_value, scaling, causal, out, workspace)
 
 
@@ -316,7 +326,13 @@ def decode_attention(query: torch.Tensor, prefix, current_key: torch.Tensor | No
     decode_workspace_bytes; one too small for the route of the call is refused.
     """
     if isinstance(prefix, PagedCache):
-        return _attend(query, prefix, prefix._desc, current_key, current_value, scaling, causal, out, workspace)
+        return prefix.attend(query, current_key, current_value, scaling=scaling, causal=causal, out=out,
+                             workspace=workspace)
+    index = query.get_device()
+    if index >= 0 and index != _lib.current_device():
+        with torch.cuda.device(index):
+            return decode_attention(query, prefix, current_key, current_value, scaling=scaling, causal=causal, out=out,
+                                    workspace=workspace)
     pre = as_prefix(prefix)
     return _attend(query, pre, None, current_key, current_value, scaling, causal, out, workspace)
 
@@ -478,7 +494,11 @@ def verify_drafts(target: torch.Tensor, draft: torch.Tensor | None, tokens: torc
     Returns (accepted [B] int32, tokens [B, K + 1] int32: the accepted drafts, the next token,
     then -1); tokens[b, accepted[b]] is -1 only when p_a has no mass.
     """
-    form = (target.shape, target.stride(), target.dtype, target.get_device(), tokens.shape, tokens.stride(), tokens.dtype,
+    index = target.get_device()
+    if index >= 0 and index != _lib.current_device():
+        with torch.cuda.device(index):
+            return verify_drafts(target, draft, tokens, counts, uniforms, workspace=workspace)
+    form = (target.shape, target.stride(), target.dtype, index, tokens.shape, tokens.stride(), tokens.dtype,
             tokens.get_device(), uniforms.shape, uniforms.stride(), uniforms.dtype, uniforms.get_device(),
             None if draft is None else (draft.shape, draft.stride(), draft.dtype, draft.get_device()),
             None if counts is None else (counts.shape, counts.stride(), counts.dtype, counts.get_device()))

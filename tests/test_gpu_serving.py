@@ -596,6 +596,52 @@ def test_one_workspace_serves_both_routes():
         assert torch.equal(cache.attend(*many, workspace=ws), want[1])
 
 
+def test_calls_make_the_tensors_device_current(monkeypatch):
+    """With another device current every call enters the tensors' own (the query of the current device
+    stands in for a second GPU); the operators that do not enter it refuse."""
+    from maskahead_b200 import _lib
+    from maskahead_b200.kernels import splitk_attention
+    from maskahead_b200.layouts import Prefix
+    from maskahead_b200.serving import PagedCache, decode_attention, verify_drafts
+
+    def calls():
+        cache = PagedCache.allocate(batch=2, heads=2, head_dim=64, num_pages=4, page_size=32, max_pages=2,
+                                    kchan=torch.ones(2, 2, 64, device=DEV))
+        q, k, v = _inputs(2, 4, 2, 2, 64, 2, seed=75)
+        plan = cache.plan(64)
+        yield lambda: plan.build(torch.tensor([20, 33], dtype=torch.int32, device=DEV)).slots
+        rows = torch.randn(64, 2, 64, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).to(DEV)
+        yield lambda: cache.append(rows, rows, plan.slots, plan.seqs, return_rows=True)[0]
+        yield lambda: cache.attend(q, k, v)
+        yield lambda: decode_attention(q, cache, k, v)
+        yield lambda: decode_attention(q, Prefix.dense(k, v), k, v)
+        yield lambda: verify_drafts(*_verify_inputs(2, 2, 50, torch.float32, seed=1))[1]
+
+    want = [f().clone() for f in calls()]
+    now, entered = [7], []
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            entered.append(self.index)
+            self.before, now[0] = now[0], self.index
+
+        def __exit__(self, *exc):
+            now[0] = self.before
+
+    with monkeypatch.context() as m:
+        m.setattr(_lib, "current_device", lambda: now[0])
+        m.setattr(torch.cuda, "device", Device)
+        got = [f().clone() for f in calls()]
+        assert entered == [0] * len(want) and now == [7]
+        q, k, v = _inputs(2, 4, 2, 2, 64, 2, seed=75)
+        with pytest.raises(RuntimeError):
+            splitk_attention(q, Prefix.dense(k, v), k, v)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_attention_refusals():
     import ctypes
 

@@ -112,6 +112,17 @@ def test_workspace_of_the_general_route(lib):
     assert lib.ma_prefix_attention_workspace(1, 1, 1, 0, 128, 0) <= _SPLITK_HEAD
 
 
+def test_launches_for_another_device_are_refused(monkeypatch):
+    """A default stream's handle is 0 on every device: the current device decides where a launch goes."""
+    from maskahead_b200 import _lib
+
+    monkeypatch.setattr(_lib, "current_device", lambda: 0)
+    monkeypatch.setattr(_lib, "_raw_stream", lambda index: 100 + index)
+    assert _lib.stream_handle(torch.device("cuda", 0)) == 100
+    with pytest.raises(RuntimeError, match="cuda:1"):
+        _lib.stream_handle(torch.device("cuda", 1))
+
+
 @pytest.mark.skipif(torch.cuda.is_available(), reason="checks the no-GPU behaviour")
 def test_no_cpu_path():
     from maskahead_b200 import KernelUnavailableError
