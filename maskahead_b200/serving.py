@@ -271,7 +271,8 @@ class PagedCache(_FixedTensors):
         if return_rows:
             rows_k = torch.empty_like(k) if k.is_contiguous() else k.new_empty(shape)
             rows_v = torch.empty_like(rows_k)
-        sk, sv = k.stride(), v.stride()
+        dense = (self.heads * self.head_dim, self.head_dim)     # (a contiguous tensor's axis of length one has any stride)
+        sk, sv = dense if k.is_contiguous() else k.stride(), dense if v.is_contiguous() else v.stride()
         rc = self._lib.ma_append_tokens(APPEND_ARGS.pack(
             k.data_ptr(), v.data_ptr(), slots.data_ptr(), seqs.data_ptr(), rows_k.data_ptr() if return_rows else 0,
             rows_v.data_ptr() if return_rows else 0, sk[0], sk[1], sv[0], sv[1], n, code, self._kv, self.batch,

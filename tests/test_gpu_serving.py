@@ -1005,6 +1005,29 @@ def test_append_strides_empty_and_refusals():
             a.append(*bad)
 
 
+@pytest.mark.parametrize("H,n", [(4, 1), (1, 3), (1, 1)])
+def test_append_axes_of_length_one_have_any_stride(H, n):
+    """A single token cut from a padded buffer, and the rows of a single head: contiguous, whatever the
+    stride of the axis of length one."""
+    from maskahead_b200.serving import PagedCache
+
+    D = 128
+    g = torch.Generator().manual_seed(80)
+    make = lambda: PagedCache.allocate(batch=1, heads=H, head_dim=D, num_pages=1, page_size=16, max_pages=1,  # noqa: E731
+                                       kchan=torch.full((1, H, D), 1.5, device=DEV))
+    if H > 1:
+        k = torch.randn(2, H * D + 1, generator=g).to(torch.bfloat16).to(DEV)[:, :H * D].unflatten(1, (H, D))[:n]
+    else:
+        k = torch.randn(n, D, generator=g).to(torch.bfloat16).to(DEV).as_strided((n, 1, D), (D, 7, 1))
+    assert k.is_contiguous() and any(s % 8 for s in k.stride()[:2])
+    slots, seqs = torch.arange(n, device=DEV), torch.zeros(n, dtype=torch.int32, device=DEV)
+    a, b = make(), make()
+    rows = a.append(k, k, slots, seqs, return_rows=True)
+    want = b.append(k.clone(memory_format=torch.contiguous_format), k.clone(memory_format=torch.contiguous_format), slots, seqs,
+                    return_rows=True)
+    assert torch.equal(a.kq, b.kq) and torch.equal(a.vz, b.vz) and torch.equal(rows[0], want[0]) and torch.equal(rows[1], want[1])
+
+
 def test_appended_tokens_are_attended():
     """Plan, append and attend agree on where a token lies."""
     from maskahead_b200.serving import PagedCache
