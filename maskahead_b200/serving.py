@@ -353,6 +353,10 @@ def _attend(query, source, desc, current_key, current_value, scaling, causal, ou
     a PagedCache remembers the forms that passed them (the checks and descriptors took 28 us
     of host time a call, the kernel of a single token over 8192 slots a third of that)."""
     forms = form = call = None
+    # plain values in the remembered forms: a tensor would be found again by its identity, whatever it holds by then
+    if scaling is not None and type(scaling) is not float:
+        scaling = float(scaling)
+    causal = bool(causal)
     if isinstance(source, PagedCache):
         forms = source._forms
         form = (query.shape, query.stride(), query.dtype, query.get_device(), scaling, causal,

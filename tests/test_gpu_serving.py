@@ -314,6 +314,19 @@ def test_peaked_and_flat_scores(scaling):
     _close(cache.attend(q, kc, vc, scaling=scaling), ref, tol)
 
 
+def test_scaling_is_read_anew_each_call():
+    """A scale (or the causal switch) given as a tensor that is written between the calls."""
+    cache = _make(2, 2, 128, [120, 45], 64, seed=81)
+    q, kc, vc = _inputs(2, 8, 2, 2, 128, 2, seed=82)
+    scale, causal = torch.tensor(0.1), torch.tensor(True)
+    for s, c in ((0.1, True), (0.02, True), (0.02, False), (1, 1)):
+        scale.fill_(s)
+        causal.fill_(c)
+        assert torch.equal(cache.attend(q, kc, vc, scaling=scale, causal=causal),
+                           cache.attend(q, kc, vc, scaling=float(scale), causal=bool(c)))
+    assert torch.equal(cache.attend(q, kc, vc, scaling=1), cache.attend(q, kc, vc, scaling=1.0))
+
+
 def test_query_magnitudes_per_row():
     """Rows from 2^-60 to 2^30: each is scaled by its own power of two (q'.k stays finite)."""
     cache = _make(1, 1, 128, [300], 64, seed=15)
