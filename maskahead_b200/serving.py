@@ -311,6 +311,11 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
     return t.clone(memory_format=torch.contiguous_format)
 
 
+def _row_strides(t: torch.Tensor) -> tuple:
+    """Strides over (b, h, t); an axis of length one is not stepped along and may have any."""
+    return tuple(s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape))
+
+
 # ----------------------------------------------------------------------------- attention
 def decode_attention(query: torch.Tensor, prefix, current_key: torch.Tensor | None = None,
                      current_value: torch.Tensor | None = None, *, scaling: float | None = None, causal: bool = True,
@@ -431,7 +436,7 @@ def _attend_form(query, source, desc, current_key, current_value, scaling, causa
                                     or current_value.device != query.device):
         raise ValueError(f"current K and V must be [{b}, {heads}, Tc, {d}] on {query.device}")
     if out is not None and (out.shape != query.shape or out.dtype != query.dtype or out.device != query.device
-                            or out.stride(-1) != 1 or any(s * out.element_size() % 16 for s in out.stride()[:3])):
+                            or out.stride(-1) != 1 or any(s * out.element_size() % 16 for s in _row_strides(out))):
         raise ValueError("out must match the query's shape, type and device, with contiguous rows on 16-byte boundaries")
     rows = hq // heads * t
     if query.dtype != torch.bfloat16 or rows > MAX_DECODE_ROWS or not (
@@ -445,7 +450,7 @@ def _attend_form(query, source, desc, current_key, current_value, scaling, causa
     none = (0, 0, 0)
     call.tail = DECODE_TAIL.pack(
         *query.stride()[:3], *(current_key.stride()[:3] if tc else none), *(current_value.stride()[:3] if tc else none),
-        *((hq * t * d, t * d, d) if out is None else out.stride()[:3]), ctypes.addressof(desc.kv), _lib.MA_BF16, b, hq,
+        *((hq * t * d, t * d, d) if out is None else _row_strides(out)), ctypes.addressof(desc.kv), _lib.MA_BF16, b, hq,
         heads, t, d, tc, 1 if causal else 0, d ** -0.5 if scaling is None else float(scaling), 0)
     call.nbytes = int(_lib.lib().ma_decode_attention_workspace(b, heads, rows, d, tc))
     return call

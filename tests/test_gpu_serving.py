@@ -354,6 +354,17 @@ def test_strides_and_out():
     assert torch.equal(cache.attend(odd, kc, vc), want)
 
 
+def test_out_axes_of_length_one_have_any_stride():
+    """One request's rows inside a padded buffer: aligned rows, whatever the stride of the axes of length one."""
+    cache = _make(1, 2, 128, [90], 64, seed=83)
+    q, kc, vc = _inputs(1, 6, 2, 1, 128, 1, seed=84)
+    want = cache.attend(q, kc, vc)
+    buf = torch.full((6 * 128 + 1,), float("nan"), device=DEV, dtype=torch.bfloat16)
+    out = buf.as_strided((1, 6, 1, 128), (769, 128, 7, 1))
+    got = cache.attend(q, kc, vc, out=out)
+    assert got is out and torch.equal(out, want) and torch.isnan(buf[-1])
+
+
 def test_tensors_are_written_into_not_replaced():
     """The calls keep the tensors' addresses: a new tensor in their place would not be read."""
     cache = _make(1, 1, 64, [10], 16, seed=60)
