@@ -414,10 +414,10 @@ def _attend_form(query, source, desc, current_key, current_value, scaling, causa
     if not query.is_cuda:
         raise _lib.KernelUnavailableError("maskahead_b200 kernels need CUDA tensors")
     b, hq, t, d = query.shape
-    tc = 0 if current_key is None else current_key.shape[2]
     if (current_key is None) != (current_value is None) or current_key is not None and (
             current_key.shape != current_value.shape or current_key.ndim != 4):
         raise ValueError("current K and V must be [B, Hkv, Tc, D] tensors of one shape")
+    tc = 0 if current_key is None else current_key.shape[2]
     if causal and 0 < tc < t:
         raise ValueError(f"causal rows need at least as many current keys as rows: Tc={tc} < T={t}")
     cached = isinstance(source, PagedCache)

@@ -666,6 +666,15 @@ def test_calls_make_the_tensors_device_current(monkeypatch):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_keys_of_another_rank_are_refused(dtype):
+    cache = _make(2, 2, 128, [50, 60], 16, seed=85)
+    q, kc, vc = (x.to(dtype) for x in _inputs(2, 4, 2, 2, 128, 2, seed=86))
+    for bad in (lambda x: x[0, 0], lambda x: x[0], lambda x: x[None]):
+        with pytest.raises(ValueError):
+            cache.attend(q, bad(kc), bad(vc))
+
+
 def test_attention_refusals():
     import ctypes
 
