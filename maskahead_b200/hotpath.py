@@ -297,7 +297,7 @@ def compact_attention(query: torch.Tensor, prefix, indices: torch.Tensor | None,
     cur, ckeep = block_struct(current_key, current_value, query.dtype)
     idx = indices if indices.dtype == torch.int64 and indices.stride(-1) == 1 else indices.to(torch.int64).contiguous()
     k = idx.shape[2]
-    out = torch.empty_like(query)
+    out = torch.empty_like(qkeep)
     nbytes = lib.ma_sparse_attention_workspace(b, hkv, (hq // hkv) * t, k, d, cur.Tc)
     ws = _lib.workspace(query.device, "attention", nbytes)
     scale = float(scaling if scaling is not None else d ** -0.5)

@@ -11,7 +11,8 @@ def _fix_inner(t: torch.Tensor) -> torch.Tensor:
     """Innermost dimension contiguous and row starts 16-byte aligned, copying if not."""
     es = t.element_size()
     ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all((s * es) % 16 == 0 for s in t.stride()[:-1])
-    return t if ok else t.contiguous()
+    # (contiguous() gives back a contiguous tensor that starts off a boundary, or whose axis of length one has an odd stride)
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
 
 
 def rows_struct(query: torch.Tensor):

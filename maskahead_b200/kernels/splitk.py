@@ -61,7 +61,7 @@ def splitk_attention(query, prefix, current_key, current_value, *, scaling=None,
     else:
         desc, kv = None, _lib.MaKV()
         kv.layout, kv.dtype = _lib.MA_KV_DENSE, rows.dtype
-    out = torch.empty_like(query)
+    out = torch.empty_like(qkeep)
     if stats_out is not None:
         mp, lp = stats_out[0], stats_out[1]
         op = stats_out[2] if len(stats_out) > 2 else None

@@ -460,6 +460,29 @@ def test_other_prefixes_take_the_general_route(kind):
     assert (got.double().cpu() - ref).norm() / ref.norm() < limit
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_general_route_copies_rows_off_a_boundary(dtype):
+    """Contiguous tensors that start between 16-byte boundaries, or whose axes of length one have odd strides."""
+    from maskahead_b200.kernels import splitk_attention
+
+    cache = _make(1, 2, 128, [90], 32, seed=87)
+    q, kc, vc = (x.to(dtype) for x in _inputs(1, 104, 2, 1, 128, 1, seed=88))
+    want = cache.attend(q, kc, vc)
+    pre = cache.prefix()
+    whole, _ = splitk_attention(q, pre, kc, vc)
+
+    def shifted(x):
+        return torch.cat([x.flatten()[:1], x.flatten()])[1:].view(x.shape)
+
+    def strided(x):
+        return x.clone().as_strided(x.shape, (x.stride(0) + 1, 128, 1, 1))
+
+    for form in (shifted, strided):
+        assert form(q).is_contiguous() and torch.equal(form(q), q)
+        assert torch.equal(cache.attend(form(q), form(kc), form(vc)), want)
+        assert torch.equal(splitk_attention(form(q), pre, form(kc), form(vc))[0], whole)
+
+
 def test_a_cache_takes_the_general_route_too():
     """float32 queries, and more rows than are read in place, over a paged cache."""
     cache = _make(2, 2, 128, [200, 90], 32, seed=30)
