@@ -443,6 +443,10 @@ MA_API int ma_prefix_attention_gather(const ma_rows* q, const ma_kv* kv, int H, 
  *   a page number outside [0, num_pages)), seqs (the request) and positions, each
  *   [max_tokens] with -1 from N on. Every output may be its input (in place); those three
  *   arrays are 16-byte aligned. B above 8192 returns MA_ERR_UNSUPPORTED.
+ * ma_live_pages: the table of a paged ma_kv (packed part only, no tail) without the page numbers
+ *   outside its pool: pages_out [B, ceil(nq / page_size)] contiguous holds each sequence's pages in
+ *   the pool, in their order, then -1; lens_out [B] the slots on them. Attention, which has no order
+ *   of slots, sees through it what the table's live slots are; neither output may be an input.
  * ma_append_tokens: N tokens' rows k, v [N, H, D] (strides over (token, head)) quantized as
  *   ma_quantize_tokens does (keys divided by kchan of sequence seqs[i]) into slots[i] of the
  *   pool (a paged token-mode ma_kv without tail; its page table is not read). A token whose
@@ -487,6 +491,7 @@ typedef struct ma_page_plan_args {
 MA_API size_t ma_page_plan_workspace(void);
 MA_API int ma_page_plan(const ma_page_plan_args* a, const int32_t* new_lens, void* workspace, size_t workspace_bytes,
                         void* stream);
+MA_API int ma_live_pages(const ma_kv* kv, int B, int32_t* pages_out, int32_t* lens_out, void* stream);
 typedef struct ma_append_args {
   const void* k;              /* [N, H, D], strides sk / sv over (token, head) */
   const void* v;

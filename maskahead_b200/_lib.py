@@ -149,6 +149,7 @@ _SIGNATURES = {
                                           _i32, _vp, _P(ctypes.c_int64), _vp, _sz, _vp]),
     "ma_page_plan_workspace": (_sz, []),
     "ma_page_plan": (_i32, [_P(MaPagePlan), _vp, _vp, _sz, _vp]),
+    "ma_live_pages": (_i32, [_P(MaKV), _i32, _vp, _vp, _vp]),
     # the argument structs of these three come packed (see the *_ARGS layouts)
     "ma_append_tokens": (_i32, [ctypes.c_char_p, _vp]),
     "ma_decode_attention_workspace": (_sz, [_i32] * 5),

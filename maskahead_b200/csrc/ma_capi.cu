@@ -902,6 +902,13 @@ int ma_page_plan(const ma_page_plan_args* a, const int32_t* new_lens, void* work
   return launch_page_plan(p, (cudaStream_t)stream);
 }
 
+int ma_live_pages(const ma_kv* kv, int B, int32_t* pages_out, int32_t* lens_out, void* stream) {
+  if (!kv || B <= 0 || kv->nq <= 0 || kv->nf != 0 || !kv->pages || kv->page_size <= 0 || kv->num_pages <= 0 || kv->spg < 0 ||
+      !pages_out || !lens_out)
+    return MA_ERR_ARG;
+  return launch_live_pages(*kv, B, pages_out, lens_out, (cudaStream_t)stream);
+}
+
 int ma_append_tokens(const ma_append_args* a, void* stream) {
   if (!a || !a->pool || a->B <= 0 || a->H <= 0 || a->N < 0) return MA_ERR_ARG;
   const ma_kv* pool = a->pool;

@@ -244,6 +244,7 @@ struct PagePlanParams {
 };
 int page_plan_max_requests();
 int launch_page_plan(PagePlanParams& p, cudaStream_t st);
+int launch_live_pages(const ma_kv& kv, int B, int32_t* pages_out, int32_t* lens_out, cudaStream_t st);
 
 // ma_append.cu: K/V rows of new tokens quantized into the slots of a packed pool
 struct AppendParams {

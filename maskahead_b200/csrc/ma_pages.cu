@@ -277,7 +277,41 @@ __global__ void __launch_bounds__(kThreads) page_plan_kernel(const __grid_consta
   }
 }
 
+// The pages that are in the pool, moved to the front of each request's table in their order, a warp
+// per request; lens_out counts their slots. A copy of the cache by this table has no dead slot below
+// its lengths, which a copy in place of the slots would have to mask.
+constexpr int kLiveWarps = 4;
+
+__global__ void __launch_bounds__(kLiveWarps * 32) live_pages_kernel(const ma_kv kv, int B, int width, int32_t* pages_out,
+                                                                      int32_t* lens_out) {
+  const int lane = threadIdx.x & 31, b = blockIdx.x * kLiveWarps + (threadIdx.x >> 5);
+  pdl_wait();
+  pdl_launch_dependents();
+  if (b >= B) return;
+  int n = kv.nq;
+  if (kv.lens != nullptr) n = min(n, max(kv.lens[b], 0));
+  const int had = (int)(((int64_t)n + kv.page_size - 1) / kv.page_size);
+  int32_t* out = pages_out + (int64_t)b * width;
+  int count = 0;
+  bool last = false;
+  for (int j0 = 0; j0 < had; j0 += 32) {
+    const int j = j0 + lane, page = j < had ? kv.pages[(int64_t)b * kv.spg + j] : -1;
+    const unsigned live = __ballot_sync(0xffffffffu, page >= 0 && page < kv.num_pages);
+    if (live >> lane & 1u) out[count + __popc(live & ((1u << lane) - 1u))] = page;
+    count += __popc(live);
+    if (had - j0 <= 32) last = live >> (had - 1 - j0) & 1u;
+  }
+  for (int j = count + lane; j < width; j += 32) out[j] = -1;
+  if (lane == 0) lens_out[b] = (int)((int64_t)count * kv.page_size - (last ? (int64_t)had * kv.page_size - n : 0));
+}
+
 }  // namespace
+
+int launch_live_pages(const ma_kv& kv, int B, int32_t* pages_out, int32_t* lens_out, cudaStream_t st) {
+  const int width = (int)(((int64_t)kv.nq + kv.page_size - 1) / kv.page_size);
+  return launch_pdl(live_pages_kernel, dim3((unsigned)((B + kLiveWarps - 1) / kLiveWarps)), dim3(kLiveWarps * 32), 0, st, kv, B,
+                    width, pages_out, lens_out) == cudaSuccess ? MA_OK : MA_ERR_CUDA;
+}
 
 int page_plan_max_requests() { return kMaxRequests; }
 

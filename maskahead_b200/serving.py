@@ -22,6 +22,7 @@ that is not read in place needs decode_workspace_bytes with its `capacity`).
 
 from __future__ import annotations
 
+import copy
 import ctypes
 
 import torch
@@ -40,7 +41,7 @@ PLAN_WORKSPACE_BYTES = 512
 # place against unpacked, device us: 32 requests x 8192 slots, 4 KV heads, 35 rows 134 / 562, 63
 # rows 178 / 564, 84 rows 280 / 567, 112 rows 374 / 331; 30 x 16000, 1 head, 96 rows 132 / 157; 4 x 8192, 4
 # heads, 112 rows 71 / 58; 1 x 8192, 35 rows 14 / 35, 84 rows 19 / 35, 112 rows 22 / 28 (and the unpacked
-# route's host time is 105 against 8).
+# route's host time is 122 against 8).
 MAX_DECODE_ROWS = 96
 
 _GROUP = 32
@@ -456,6 +457,28 @@ def _attend_form(query, source, desc, current_key, current_value, scaling, causa
     return call
 
 
+def _without_dead_pages(prefix: Prefix, batch: int, heads: int, head_dim: int, desc) -> Prefix:
+    """The paged prefix as the unpacked copy may hold it: that copy has no page table, so slots on
+    page numbers outside the pool would come back as keys of zeros. Their pages are left out (the
+    order of slots does not matter to attention), or, where slots are named by a mask or a tail's
+    place behind them, masked."""
+    own, nq, dev = copy.copy(prefix), prefix.nq, prefix.vq.device
+    if prefix.mask is None and prefix.nf == 0:
+        width = -(-nq // prefix.page_size)
+        words = torch.empty(batch * (width + 1), device=dev, dtype=torch.int32)
+        own.pages, own.lens = words[batch:].view(batch, width), words[:batch]
+        if desc is None:
+            desc = kv_descriptor(prefix, batch=batch, heads=heads, head_dim=head_dim)
+        _lib.check("ma_live_pages", _lib.lib().ma_live_pages(desc.kv, batch, own.pages.data_ptr(), own.lens.data_ptr(),
+                                                             _lib.stream_handle(dev)))
+        return own
+    live = (prefix.pages >= 0) & (prefix.pages < prefix.vq.shape[0])
+    live = live[:, torch.arange(nq, device=dev) // prefix.page_size]
+    live = torch.cat([live, live.new_ones(batch, prefix.nf)], 1)[:, None].expand(batch, heads, prefix.n)
+    own.mask = live.contiguous() if prefix.mask is None else live & prefix.mask.bool()
+    return own
+
+
 def _attend_general(query, source, current_key, current_value, scaling, causal, out, workspace):
     from .hotpath import unpacked_prefix
     from .kernels.splitk import splitk_attention
@@ -478,6 +501,8 @@ def _attend_general(query, source, current_key, current_value, scaling, causal, 
             at_v = at_k + ((size + 255) & ~255)
             unpacked = tuple(workspace[x:x + size].view(torch.bfloat16).view(shape) for x in (at_k, at_v))
     if unpack:
+        if prefix.pages is not None:
+            prefix = _without_dead_pages(prefix, b, heads, d, source._desc if isinstance(source, PagedCache) else None)
         prefix = unpacked_prefix(prefix, b, heads, d, out=unpacked)
     res, _ = splitk_attention(query, prefix, current_key, current_value, scaling=scaling,
                               causal_block=1 if causal and tc else 0, q_pos0=tc - t, c_pos0=0, workspace=scratch)

@@ -460,6 +460,42 @@ def test_other_prefixes_take_the_general_route(kind):
     assert (got.double().cpu() - ref).norm() / ref.norm() < limit
 
 
+@pytest.mark.parametrize("D,page", [(128, 64), (128, 16), (64, 48)])
+@pytest.mark.parametrize("kind", ["plain", "no lens", "mask", "tail"])
+def test_bad_pages_read_as_dead_on_the_general_route(kind, D, page):
+    """More rows than are read in place: page numbers outside the pool stay dead in the unpacked copy too."""
+    from maskahead_b200.serving import decode_attention
+
+    B, H, T = 4, 2, 2
+    lens = [300, 223, 0, 1500]
+    cache = _make(B, H, D, lens, page, seed=89)
+    pre = cache.prefix()
+    cache.pages[0, 2] = -1
+    cache.pages[0, (lens[0] - 1) // page] = cache.num_pages            # the last, partial page
+    cache.pages[1, 0] = 2 ** 30
+    cache.pages[3, 5:23:3] = -7
+    q, kc, vc = _inputs(B, 104, H, T, D, T, seed=90)
+    if kind == "no lens":                                             # every slot of the table
+        pre.lens = None
+        cache.ks.nan_to_num_(0.0), cache.kz.nan_to_num_(0.0), cache.vs.nan_to_num_(0.0), cache.vz.nan_to_num_(0.0)
+    if kind == "mask":
+        g = torch.Generator().manual_seed(91)
+        pre.mask = (torch.rand(B, H, pre.nq, generator=g) < 0.7).to(DEV)
+    if kind == "tail":                                                # bf16 rows behind the paged part: full tables
+        pre.lens, m = None, 33
+        cache.ks.nan_to_num_(0.0), cache.kz.nan_to_num_(0.0), cache.vs.nan_to_num_(0.0), cache.vz.nan_to_num_(0.0)
+        tk, tv = _inputs(B, H, H, 1, D, m, seed=92)[1:]
+        ref, _ = _attend_ref(q, pre, torch.cat([tk, kc], 2), torch.cat([tv, vc], 2))
+        pre.kf, pre.vf, pre.nf = tk, tv, m
+    else:
+        ref, _ = _attend_ref(q, pre, kc, vc)
+    out = decode_attention(q, pre, kc, vc)
+    assert torch.isfinite(out).all()
+    assert (out.double() - ref).norm() <= 2e-2 * ref.norm()           # as test_many_rows
+    if kind == "plain":
+        assert torch.equal(cache.attend(q, kc, vc), out)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_general_route_copies_rows_off_a_boundary(dtype):
     """Contiguous tensors that start between 16-byte boundaries, or whose axes of length one have odd strides."""

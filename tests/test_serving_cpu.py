@@ -54,6 +54,20 @@ def test_rejected_arguments(lib):
     assert lib.ma_verify_drafts(_verify(ws=4096, nbytes=1000), None) == -3
 
 
+def test_live_pages_rejects_what_has_no_table(lib):
+    from maskahead_b200._lib import MaKV
+
+    assert lib.ma_live_pages(None, 1, 16, 16, None) == -1
+    kv = MaKV()
+    kv.nq = 32
+    assert lib.ma_live_pages(kv, 1, 16, 16, None) == -1               # not paged
+    kv.pages, kv.page_size, kv.num_pages = 16, 16, 4
+    for b, out, lens in ((0, 16, 16), (1, None, 16), (1, 16, None)):
+        assert lib.ma_live_pages(kv, b, out, lens, None) == -1
+    kv.nf = 1
+    assert lib.ma_live_pages(kv, 1, 16, 16, None) == -1               # a tail behind the table
+
+
 def test_packed_structs_match_the_header(tmp_path):
     """The packed argument structs have the sizes and offsets that a C compiler gives the header's."""
     import shutil
