@@ -777,7 +777,16 @@ __global__ void __launch_bounds__(W * 32, MINB) decode_attention_kernel(const __
         for (int i = 0; i < 8; ++i) o[nt][gr][i] = 0.f;
     }
     bool first = true;               // no live tile yet: off is not set
-    int fe = 0;                      // V scales are used times 2^fe, so that none reaches 2
+    uint32_t power[NG / 2];          // V scales are used times a power of two per group (fp16, two to a word), so that none reaches 2
+#pragma unroll
+    for (int e = 0; e < NG / 2; ++e) power[e] = 0x3C003C00u;
+    auto power_of = [&](int gr) { return (int)(power[gr / 2] >> (16 * (gr & 1) + 10) & 31u) - 15; };
+    auto any_power = [&]() {
+      uint32_t x = 0u;
+#pragma unroll
+      for (int e = 0; e < NG / 2; ++e) x |= power[e] ^ 0x3C003C00u;
+      return x != 0u;
+    };
     uint32_t stage = ring;           // ring stage of tile i
 #pragma unroll 1
     for (int i = warp; i < tiles; i += W) {
@@ -896,38 +905,45 @@ __global__ void __launch_bounds__(W * 32, MINB) decode_attention_kernel(const __
             for (int e = 0; e < 8; ++e) o[nt][gr][e] *= corr[e & 1];
         }
       }
-      if (__any_sync(0xffffffffu, (vtop & 0x40004000u) != 0u) || fe != 0 || first) {
-        // the exponent of the tile's largest V scale; from then on the scales are brought below 2 (fp16
-        // products p * scale stay finite), and up to it if a sequence begins with scales below 2^-6
-        // (they stay out of fp16's subnormals)
+      if (__any_sync(0xffffffffu, (vtop & 0x40004000u) != 0u) || any_power() || first) {
+        // The scales of a group are brought below 2 (fp16 products p * scale stay finite), and all of them up to
+        // it if a sequence begins with scales below 2^-6 (they stay out of fp16's subnormals). Each group has
+        // its own power: one of large values must not push another's scales below what fp16 holds (values
+        // of 1000 beside 0.001 with one power: 4 % of the latter's output).
         const uint32_t va = st + R::kVs + lane * kSc;
-        uint32_t top;
-        if constexpr (NG == 4) {
-          const uint2 u = lds64(va);
-          const uint32_t a = __vmaxu2(u.x & 0x7fff7fffu, u.y & 0x7fff7fffu);
-          top = max(a & 0xffffu, a >> 16);
-        } else {
-          const uint32_t a = lds32(va) & 0x7fff7fffu;
-          top = max(a & 0xffffu, a >> 16);
+        uint32_t u[NG / 2], reach = first ? 0x40004000u : 0u;
+#pragma unroll
+        for (int e = 0; e < NG / 2; ++e) {
+          u[e] = lds32(va + e * 4);
+          reach |= hmul2(u[e], power[e]);
         }
-        const int e5 = min(max((int)(__reduce_max_sync(0xffffffffu, top) >> 10), 1), 30);
-        int to = min(fe, 15 - e5);
-        if (first) to = e5 < 9 || e5 > 15 ? 15 - e5 : 0;
-        if (to != fe) {
-          const float down = __uint_as_float((uint32_t)(127 + to - fe) << 23);
+        if (__any_sync(0xffffffffu, (reach & 0x40004000u) != 0u)) {
+          int e5[NG], most = 1;                // exponents of the groups' largest scales in the tile
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+          for (int gr = 0; gr < NG; ++gr) {
+            const uint32_t x = u[gr / 2] >> (16 * (gr & 1)) & 0x7fffu;
+            e5[gr] = min(max((int)(__reduce_max_sync(0xffffffffu, x) >> 10), 1), 30);
+            most = max(most, e5[gr]);
+          }
+          const int up = most < 9 ? 15 - most : 0;
 #pragma unroll
-            for (int gr = 0; gr < NG; ++gr)
+          for (int gr = 0; gr < NG; ++gr) {
+            const int is = power_of(gr), to = min(first ? up : is, 15 - e5[gr]);
+            if (to != is) {
+              const float down = __uint_as_float((uint32_t)(127 + to - is) << 23);
 #pragma unroll
-              for (int e = 0; e < 8; ++e) o[nt][gr][e] *= down;
-          fe = to;
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o[nt][gr][e] *= down;
+              const uint32_t half = to > -15 ? (uint32_t)(to + 15) << 10 : 0x0200u;
+              power[gr / 2] = gr & 1 ? __byte_perm(power[gr / 2], half, 0x5410) : __byte_perm(half, power[gr / 2], 0x7610);
+            }
+          }
         }
-        if (fe != 0) {
-          const uint32_t fh = fe > -15 ? (uint32_t)(fe + 15) << 10 : 0x0200u, f2 = fh | fh << 16;
+        if (any_power()) {
           __syncwarp();
 #pragma unroll
-          for (int e = 0; e < NG / 2; ++e) sts32(va + e * 4, hmul2(lds32(va + e * 4), f2));
+          for (int e = 0; e < NG / 2; ++e) sts32(va + e * 4, hmul2(u[e], power[e]));
           __syncwarp();
         }
       }
@@ -1028,7 +1044,6 @@ __global__ void __launch_bounds__(W * 32, MINB) decode_attention_kernel(const __
     __syncthreads();
 
     // ---- the warps' rows to shared memory (over the rings): o = codes' part + zeros' part
-    const float unit = __uint_as_float((uint32_t)(127 + 24 - (int)kUp - fe) << 23);
     constexpr float kZ = 1.f / 256.f;     // 2^-kUp
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -1041,6 +1056,7 @@ __global__ void __launch_bounds__(W * 32, MINB) decode_attention_kernel(const __
       for (int gr = 0; gr < NG; ++gr) {
         const float za = __shfl_sync(0xffffffffu, z[nt][0], 4 * gr + t4) * kZ;
         const float zc = __shfl_sync(0xffffffffu, z[nt][1], 4 * gr + t4) * kZ;
+        const float unit = __uint_as_float((uint32_t)(127 + 24 - (int)kUp - power_of(gr)) << 23);
         const float* oo = o[nt][gr];
         const int d = 32 * gr + 4 * g;
         *reinterpret_cast<float4*>(row + d) =

@@ -293,6 +293,31 @@ def test_value_ranges(vscale):
     _close(cache.attend(q), ref, tol)
 
 
+@pytest.mark.parametrize("D", [128, 64])
+@pytest.mark.parametrize("small,large", [(1e-4, 1e3), (1e-2, 1e4), (1e-3, 1e-1)])
+@pytest.mark.parametrize("late", [False, True])
+def test_value_groups_of_different_sizes(D, small, large, late):
+    """A channel group of large values (from the start, or from the middle on) leaves the others exact to
+    the same relative bounds."""
+    n = 600
+    cache = _make(1, 1, D, [n], 64, seed=93)
+    g = torch.Generator().manual_seed(94)
+    v = torch.randn(1, n, D, generator=g) * small
+    v[:, n // 2 if late else 0:, 32:64] *= large / small
+    pv, sv, zv = _packed_rows(v)
+    for i, page in enumerate(cache.pages[0].tolist()):
+        lo, hi = i * 64, min(n, i * 64 + 64)
+        for t, x in ((cache.vq, pv), (cache.vs, sv), (cache.vz, zv)):
+            t[page, :, :hi - lo] = x[:, lo:hi].to(DEV)
+    q, _, _ = _inputs(1, 16, 1, 1, D, 0, seed=95)
+    ref, tol = _attend_ref(q, cache.prefix(), None, None)
+    out = cache.attend(q)
+    _close(out, ref, tol)
+    for first in range(0, D, 32):
+        part = slice(first, first + 32)
+        assert (out[..., part].double() - ref[..., part]).norm() <= 3e-3 * ref[..., part].norm()
+
+
 def test_zero_value_scales():
     """A group of equal values has scale 1e-8, which fp16 rounds to 0."""
     cache = _make(1, 1, 128, [100], 16, seed=13)
