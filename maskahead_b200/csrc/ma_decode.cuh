@@ -133,6 +133,10 @@ __device__ __forceinline__ void add2(float& a0, float& a1, float b0, float b1) {
   asm("{\n.reg .b64 x, y;\nmov.b64 x, {%0, %1};\nmov.b64 y, {%2, %3};\nadd.rn.f32x2 x, x, y;\nmov.b64 {%0, %1}, x;\n}\n"
       : "+f"(a0), "+f"(a1) : "f"(b0), "f"(b1));
 }
+__device__ __forceinline__ void mul2(float& a0, float& a1, float b0, float b1) {
+  asm("{\n.reg .b64 x, y;\nmov.b64 x, {%0, %1};\nmov.b64 y, {%2, %3};\nmul.rn.f32x2 x, x, y;\nmov.b64 {%0, %1}, x;\n}\n"
+      : "+f"(a0), "+f"(a1) : "f"(b0), "f"(b1));
+}
 // (a0, a1) += (c0, c1) * (b0, b1)
 __device__ __forceinline__ void fma2(float& a0, float& a1, float c0, float c1, float b0, float b1) {
   asm("{\n.reg .b64 x, y, z;\nmov.b64 x, {%0, %1};\nmov.b64 y, {%2, %3};\nmov.b64 z, {%4, %5};\nfma.rn.f32x2 x, y, z, x;\n"
@@ -494,10 +498,12 @@ __device__ __forceinline__ void stage_query(const DecodeParams& p, const QueryLo
                                  pack_half2(x[gr][2], x[gr][6]), pack_half2(x[gr][3] * 0.0625f, x[gr][7] * 0.0625f));
     z += __shfl_xor_sync(0xffffffffu, z, 1);
     z += __shfl_xor_sync(0xffffffffu, z, 2);
-    zg[gr] = z * 5.9604645e-8f;  // 2^-24, the unit of the codes' products
+    zg[gr] = z * 0.03125f;       // below 2^14
   }
-  // the groups' sums of q' for the zero term, as fp16 high and low parts: together exact to
-  // half a unit of q', below q's own rounding
+  // the groups' sums of q' for the zero term, as fp16 high and low parts: together good to 2^-21 of a sum
+  // or 2^-20 of the unit of q', so that a group of small q' keeps its part of a score when its zeros are
+  // large. (In the codes' unit, 2^-24, the low parts were subnormal: with q' 100 times smaller in the
+  // groups whose keys are 100 times larger, and the other way round, outputs were off by 3 %.)
   float z0, z1;
   bool low;
   if constexpr (NG == 4) {
@@ -811,7 +817,12 @@ __global__ void __launch_bounds__(W * 32, MINB) decode_attention_kernel(const __
         const uint32_t za = st + R::kKz + (2 * g + mt) * kSc + (NG == 4 ? (t4 & 1) * 4 : 0);
         const uint32_t z0 = lds32(za), z1 = lds32(za + 16 * kSc);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma8(sc[mt][nt], z0, z1, zb[nt]);
+        for (int nt = 0; nt < NT; ++nt) {
+          constexpr float kToCodes = 1.9073486e-6f;      // 2^-19: to the codes' unit
+          mma8(sc[mt][nt], z0, z1, zb[nt]);
+          mul2(sc[mt][nt][0], sc[mt][nt][1], kToCodes, kToCodes);
+          mul2(sc[mt][nt][2], sc[mt][nt][3], kToCodes, kToCodes);
+        }
       }
 #pragma unroll
       for (int gp = 0; gp < NG / 2; ++gp) {

@@ -318,6 +318,28 @@ def test_value_groups_of_different_sizes(D, small, large, late):
         assert (out[..., part].double() - ref[..., part]).norm() <= 3e-3 * ref[..., part].norm()
 
 
+@pytest.mark.parametrize("D", [128, 64])
+@pytest.mark.parametrize("ratio", [10.0, 100.0, 1000.0])
+def test_query_and_key_groups_of_opposite_sizes(D, ratio):
+    """Channels whose queries are as much smaller as their keys (with large zeros) are larger give their
+    whole part of a score."""
+    n = 600
+    cache = _make(1, 1, D, [n], 64, seed=96)
+    g = torch.Generator().manual_seed(97)
+    size = torch.full((D,), 1 / ratio)
+    size[32:64] = ratio
+    pk, sk, zk = _packed_rows((torch.randn(1, n, D, generator=g) + 2) * size)
+    for i, page in enumerate(cache.pages[0].tolist()):
+        lo, hi = i * 64, min(n, i * 64 + 64)
+        for t, x in ((cache.kq, pk), (cache.ks, sk), (cache.kz, zk)):
+            t[page, :, :hi - lo] = x[:, lo:hi].to(DEV)
+    cache.kchan.fill_(1.0)
+    q, _, _ = _inputs(1, 16, 1, 1, D, 0, seed=98)
+    q = (q.float() / size.to(DEV)).to(torch.bfloat16)
+    ref, tol = _attend_ref(q, cache.prefix(), None, None)
+    _close(cache.attend(q), ref, tol)
+
+
 def test_zero_value_scales():
     """A group of equal values has scale 1e-8, which fp16 rounds to 0."""
     cache = _make(1, 1, 128, [100], 16, seed=13)
