@@ -23,11 +23,11 @@ bool contiguous_tiles(const ma_kv& kv, int D) {
 
 // Rows per tile: a tile of more rows unpacks the codes fewer times, but 24 and 32 rows leave
 // registers for 8 warps an SM only. 32 requests x 8192 slots, 4 KV heads, D = 128 (D = 64), us:
-//   14 rows: 16 -> 60 (39), 24 -> 78 (51), 32 -> 99 (60)
-//   21 rows: 16 -> 98 (67), 24 -> 82 (53), 32 -> 103 (62)
-//   28 rows: 16 -> 99 (69), 24 -> 134 (89), 32 -> 109 (67)
-//   35 rows: 16 -> 150 (92), 24 -> 134 (89), 32 -> 176 (107)
-//   56 rows: 16 -> 197 (129), 24 -> 209 (140), 32 -> 180 (111)
+//   14 rows: 16 -> 59 (39), 24 -> 76 (50), 32 -> 98 (57)
+//   21 rows: 16 -> 99 (67), 24 -> 81 (54), 32 -> 104 (61)
+//   28 rows: 16 -> 100 (68), 24 -> 133 (88), 32 -> 107 (62)
+//   35 rows: 16 -> 150 (93), 24 -> 135 (90), 32 -> 181 (103)
+//   56 rows: 16 -> 194 (127), 24 -> 208 (140), 32 -> 184 (106)
 // The general form has no 24-row tile.
 int rows_per_tile(int R, int D, bool has24) {
   if (R <= 8) return 8;

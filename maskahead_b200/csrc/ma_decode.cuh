@@ -20,7 +20,7 @@
 // D = 128).
 //
 // Measured, D = 128, 4 KV heads: 64 requests of 4096 to 16384 slots, 7 rows, 89 us (421 MB: 4.7 TB/s, 73%
-// of a copy's rate); 32 such requests, 35 rows, 166 us; 1 request, 8192 slots, 10.4 us, of which the
+// of a copy's rate); 32 such requests, 35 rows, 168 us; 1 request, 8192 slots, 10.7 us, of which the
 // chain lengths -> page table -> tiles -> merge takes all but a microsecond or two.
 //
 // A warp owns 32-slot tiles and a private ring of shared memory filled by cp.async (16-byte

@@ -381,7 +381,7 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant_
 
 int verify_max_requests() { return kMaxRequests; }
 
-// About 9 CTAs of 4 warps an SM, at least one a request: more than are resident at once (5),
+// About 9 CTAs of 4 warps an SM, at least one a request: more than are resident at once (6),
 // because a refused draft doubles a request's bytes and later CTAs even that out. A warp's share
 // is whole spans.
 void plan_verify(int B, int V, int elem, VerifyPlan& plan) {

@@ -38,10 +38,11 @@ PLAN_WORKSPACE_BYTES = 512
 
 # Rows per KV head (query heads of the group x tokens) up to which attention reads the packed
 # cache in place; beyond, a prefix is unpacked once and the 128-row tensor-core tiles run. In
-# place against unpacked, device us: 32 requests x 8192 slots, 4 KV heads, 35 rows 134 / 562, 63
-# rows 178 / 564, 84 rows 280 / 567, 112 rows 374 / 331; 30 x 16000, 1 head, 96 rows 132 / 157; 4 x 8192, 4
-# heads, 112 rows 71 / 58; 1 x 8192, 35 rows 14 / 35, 84 rows 19 / 35, 112 rows 22 / 28 (and the unpacked
-# route's host time is 122 against 8).
+# place against unpacked, device us: 32 requests x 8192 slots, 4 KV heads, 35 rows 134 / 563, 63
+# rows 186 / 565, 84 rows 288 / 567, 112 rows 371 / 334; 30 x 16000, 1 head, 96 rows 135 / 161; 4 x 8192, 4
+# heads, 84 rows 48 / 86, 112 rows 72 / 60; 1 x 8192, 84 rows 19 / 37, 112 rows 22 / 29, 224 rows 47 / 29; 1 x 300,
+# 112 rows 12 / 17, 224 rows 19 / 17. The unpacked route's host time is 122 against 8, so a short call just
+# past the constant is the slower one: it is one number for all sizes.
 MAX_DECODE_ROWS = 96
 
 _GROUP = 32
